@@ -215,6 +215,61 @@ int ptts_b200_attend(ptts_b200_kv* kv, int layer, const void* q, const void* k, 
                      int out_dtype, void* cuda_stream);
 
 /* ---------------------------------------------------------------------------------------
+ * Attention with score rules, and drafted trees. No counterpart in the reference: for models
+ * whose scores are capped or carry a distance bias, for rows that see a span of positions
+ * (documents packed in one stream, a prefix that sees itself whole, a window, padding rows), and
+ * for sessions that draft several rows ahead and keep a path of them.
+ *
+ * With s_j = q . k_j / sqrt(64) over the positions j that a row at position p sees:
+ *   t_j = softcap * tanh(s_j / softcap)    (s_j where softcap is 0)
+ *   u_j = t_j - slopes[head] * |p - j|     (t_j where slopes is NULL)
+ *   out = sum_j exp(u_j) v_j / sum_j exp(u_j), and zeros for a row that sees nothing.
+ * Keys that a row does not see never reach its output, whatever they hold (NaN included).
+ * ------------------------------------------------------------------------------------- */
+typedef struct {
+    float softcap;         /* positive, or 0 for none */
+    const float* slopes;   /* [num_heads] f32 (device), or NULL */
+    const int32_t* first;  /* [n_rows] (device): the first position a row sees; NULL: 0 */
+    const int32_t* last;   /* [n_rows] (device): the last position a row sees; NULL: its own */
+} ptts_b200_scores;
+
+/* ptts_b200_attend with score rules (`scores` may be NULL: none): the same rows, append and
+ * output, each row seeing the positions first..last, clamped to 0 .. length + rows - 1 of its
+ * stream; first > last sees nothing. A causal document mask is first = the document's start; a
+ * prefix mask is last = max(position, prefix - 1); a window of w is first = position - w + 1.
+ * max_period 0 leaves q and k unrotated (for a distance bias in place of RoPE).
+ * q, k, v and out are aligned to 16 bytes. Streams are appended streams (rings and windowed
+ * streams are refused with PTTS_B200_ERR_UNSUPPORTED), and the call cannot be captured in a CUDA
+ * graph (PTTS_B200_ERR_STATE): it plans from the host's lengths. Lengths are not advanced. */
+int ptts_b200_attend_scored(ptts_b200_kv* kv, int layer, const void* q, const void* k, const void* v,
+                            int in_dtype, int num_kv_heads, const int32_t* streams_host,
+                            const int32_t* rows_host, int n_seq, float max_period,
+                            const ptts_b200_scores* scores, void* out, int out_dtype,
+                            void* cuda_stream);
+
+/* Attention of drafted trees over the cache: sequence i drafts rows_host[i] nodes (at most 64) on
+ * its stream. parents [n_rows] (device): a node's parent as an index within its sequence, below
+ * its own, or -1 for a root. A node sees the cached positions 0 .. length - 1, its ancestors and
+ * itself; it sits at position length + depth (rotation and bias), and its k and v are written to
+ * slot length + index. scores->first limits both to positions from it on; scores->last must be
+ * NULL. A parent out of range refuses its sequence on the device (PTTS_B200_DEVERR_BOUNDS in
+ * ptts_b200_kv_check): nothing is written to its slots and its output rows are zeros. Otherwise
+ * as ptts_b200_attend_scored. */
+int ptts_b200_attend_tree(ptts_b200_kv* kv, int layer, const void* q, const void* k, const void* v,
+                          int in_dtype, int num_kv_heads, const int32_t* streams_host,
+                          const int32_t* rows_host, int n_seq, const int32_t* parents, float max_period,
+                          const ptts_b200_scores* scores, void* out, int out_dtype, void* cuda_stream);
+
+/* Keep a path of each stream's drafted tree, after the last layer's ptts_b200_attend_tree: the
+ * rows of the accepted nodes (nodes_host: counts_host[i] of them for stream streams_host[i], one
+ * stream's after another's, rising: a root, a child of it, ...) move to the slots behind the
+ * cached rows in every layer, and the stream's length grows by their number. A count may be 0.
+ * Refused as a whole, before anything changes: a stream named twice, nodes that do not rise within
+ * 0..63, a node outside the capacity, rings and windowed streams, capture in a CUDA graph. */
+int ptts_b200_kv_accept(ptts_b200_kv* kv, const int32_t* streams_host, const int32_t* counts_host,
+                        const int32_t* nodes_host, int n, void* cuda_stream);
+
+/* ---------------------------------------------------------------------------------------
  * Quantised linear: Q::LinearQ::forward (transformer.rs:195, :224, :627) for int8 weights with
  * one f32 scale per output row. y[m][n] = scale[n] * sum_k x[m][k] * w[n][k].
  * x [m][k] bf16, w [n][k] int8, scale [n] f32, y [m][n] f32; all device pointers.

@@ -5,6 +5,8 @@ surface for this path:
 
     KvState       StreamingTransformerState (ptts/src/transformer.rs:328-393)
     attend        StreamingMultiheadAttention::forward after in_proj (transformer.rs:197-248)
+    attend_scored attend with capped scores, a distance bias and per-row spans (no counterpart)
+    attend_tree   attention of drafted trees over the cache (no counterpart; KvState.accept)
     linear_i8     Q::LinearQ::forward with int8 per-output-channel weights
     Transformer   StreamingTransformer::{forward, forward_step} (transformer.rs:742-838)
 
@@ -50,6 +52,7 @@ EXPORTS = (
     "ptts_b200_model_config", "ptts_b200_model_load_layer_f32", "ptts_b200_model_load_layer_q8_0",
     "ptts_b200_load_gguf", "ptts_b200_gguf_remap_key", "ptts_b200_kv_set_window",
     "ptts_b200_model_stamps", "ptts_b200_model_stamps_read", "ptts_b200_model_set_layer_scale",
+    "ptts_b200_attend_scored", "ptts_b200_attend_tree", "ptts_b200_kv_accept",
 )
 
 
@@ -86,6 +89,12 @@ class LayerWeightsF32(ctypes.Structure):
 class LayerWeightsQ8(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in (
         "in_proj", "out_proj", "linear1", "linear2", "norm1_weight", "norm1_bias", "norm2_weight", "norm2_bias")]
+
+
+class Scores(ctypes.Structure):
+    """ptts_b200_scores: the score rules of attend_scored and attend_tree."""
+    _fields_ = [("softcap", ctypes.c_float), ("slopes", ctypes.c_void_p), ("first", ctypes.c_void_p),
+                ("last", ctypes.c_void_p)]
 
 
 class FlowConfigC(ctypes.Structure):
@@ -151,6 +160,9 @@ def lib() -> ctypes.CDLL:
         L.ptts_b200_kv_copy_stream.argtypes = [P, I, P, I, P]
         L.ptts_b200_kv_check.argtypes = [P]
         L.ptts_b200_attend.argtypes = [P, I, P, P, P, I, I, IP, IP, I, F, P, I, P]
+        L.ptts_b200_attend_scored.argtypes = [P, I, P, P, P, I, I, IP, IP, I, F, ctypes.POINTER(Scores), P, I, P]
+        L.ptts_b200_attend_tree.argtypes = [P, I, P, P, P, I, I, IP, IP, I, P, F, ctypes.POINTER(Scores), P, I, P]
+        L.ptts_b200_kv_accept.argtypes = [P, IP, IP, IP, I, P]
         L.ptts_b200_linear_i8.argtypes = [I, P, P, P, I, I, I, P, P]
         L.ptts_b200_model_create.argtypes = [I, ctypes.POINTER(Config), ctypes.POINTER(P)]
         L.ptts_b200_model_destroy.argtypes = [P]
@@ -214,6 +226,16 @@ def _stream(stream=None) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def _stream_of(device: int, stream=None) -> ctypes.c_void_p:
+    """The CUDA stream handle for a call on `device`, which need not be the current one: `stream`'s,
+    else torch's current stream there."""
+    import torch
+    if stream is not None:
+        return ctypes.c_void_p(stream.cuda_stream)
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return ctypes.c_void_p(raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream)
+
+
 def _dptr(t) -> ctypes.c_void_p:
     if not t.is_cuda:
         raise PttsError(ERR_ARG, "expected a CUDA tensor")
@@ -232,9 +254,11 @@ def _dtype_code(t) -> int:
 
 
 class _Cai:
-    """A raw device buffer exposed through __cuda_array_interface__ (for torch.as_tensor)."""
+    """A raw device buffer exposed through __cuda_array_interface__ (for torch.as_tensor, whose
+    tensor holds this object and with it the buffer's `owner`)."""
 
-    def __init__(self, ptr: int, shape, typestr: str):
+    def __init__(self, ptr: int, shape, typestr: str, owner=None):
+        self.owner = owner
         self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": typestr,
                                          "data": (ptr, False), "version": 3, "strides": None}
 
@@ -327,19 +351,20 @@ class KvState:
     def tensors(self, layer: int):
         """Views (torch, no copy) of one layer's K and V caches and the device lengths [S]: the
         caches as [S, cap, H, D] with 8 heads, and as [S, cap, H / 8, 8, D] with more (each
-        group of 8 heads is its own [S, cap, 8, D] block; `.reshape(S, cap, H, D)` copies)."""
+        group of 8 heads is its own [S, cap, 8, D] block; `.reshape(S, cap, H, D)` copies). The
+        views keep this state alive (until `close`)."""
         import torch
         k, v, ln = self.pointers(layer)
         G = self.num_heads // 8
         shape = (G, self.num_streams, self.capacity, 8, self.head_dim)
         if self.dtype == "bf16":
-            kt = torch.as_tensor(_Cai(k, shape, "<i2"), device=f"cuda:{self.device}").view(torch.bfloat16)
-            vt = torch.as_tensor(_Cai(v, shape, "<i2"), device=f"cuda:{self.device}").view(torch.bfloat16)
+            kt = torch.as_tensor(_Cai(k, shape, "<i2", self), device=f"cuda:{self.device}").view(torch.bfloat16)
+            vt = torch.as_tensor(_Cai(v, shape, "<i2", self), device=f"cuda:{self.device}").view(torch.bfloat16)
         else:
-            kt = torch.as_tensor(_Cai(k, shape, "<f4"), device=f"cuda:{self.device}")
-            vt = torch.as_tensor(_Cai(v, shape, "<f4"), device=f"cuda:{self.device}")
+            kt = torch.as_tensor(_Cai(k, shape, "<f4", self), device=f"cuda:{self.device}")
+            vt = torch.as_tensor(_Cai(v, shape, "<f4", self), device=f"cuda:{self.device}")
         kt, vt = (t[0] if G == 1 else t.permute(1, 2, 0, 3, 4) for t in (kt, vt))
-        lt = torch.as_tensor(_Cai(ln, (self.num_streams,), "<i4"), device=f"cuda:{self.device}")
+        lt = torch.as_tensor(_Cai(ln, (self.num_streams,), "<i4", self), device=f"cuda:{self.device}")
         return kt, vt, lt
 
     def load_prefix(self, layer: int, stream: int, k, v, set_length: bool = True, cuda_stream=None):
@@ -369,6 +394,17 @@ class KvState:
             out.copy_stream(s, self, s)
         return out
 
+    def accept(self, streams: Sequence[int], nodes: Sequence[Sequence[int]], stream=None):
+        """Keep the drafted nodes `nodes[i]` (rising indexes, a path of attend_tree's tree; may be
+        empty) of stream `streams[i]`: their rows move behind the cached ones in every layer, and
+        the stream grows by their number (ptts_b200_kv_accept)."""
+        if len(nodes) != len(streams):
+            raise PttsError(ERR_ARG, "one path per stream")
+        st, flat = _i32(streams), _i32([x for path in nodes for x in path])
+        counts = _i32([len(path) for path in nodes])
+        _check(lib().ptts_b200_kv_accept(self._h, _ip(st), _ip(counts), _ip(flat), len(st),
+                                         _stream_of(self.device, stream)))
+
     def check(self):
         """Raise if a kernel's own bounds check or bounded wait tripped (synchronises)."""
         _check(lib().ptts_b200_kv_check(self._h))
@@ -397,6 +433,84 @@ def attend(kv: KvState, layer: int, q, k, v, streams: Sequence[int], rows: Seque
                                   int(k.shape[1]), _ip(s), _ip(r), len(s), max_period, _dptr(out),
                                   _dtype_code(out), _stream(stream)))
     return out
+
+
+def _rule_tensor(kv: KvState, t, name: str, dtype, n: int):
+    """The device pointer of a rule's vector (None: NULL), checked."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise PttsError(ERR_ARG, f"{name} must be a contiguous vector of {n} {dtype}")
+    if t.device.type != "cuda" or t.device.index != kv.device:
+        raise PttsError(ERR_ARG, f"{name} must be on cuda:{kv.device}, where the cache is")
+    return t.data_ptr()
+
+
+def _attend_rules(kv: KvState, layer, q, k, v, streams, rows, parents, tree, softcap, slopes, first, last, max_period,
+                  out_dtype, out, stream):
+    import torch
+    if q.dtype != k.dtype or q.dtype != v.dtype:
+        raise PttsError(ERR_ARG, "q, k and v must share a dtype")
+    code = _dtype_code(q)
+    s, r = _i32(streams), _i32(rows)
+    if s.ndim != 1 or s.shape != r.shape:
+        raise PttsError(ERR_ARG, "one row count per stream")
+    n, H, D = int(r.sum()), kv.num_heads, kv.head_dim
+    if q.dim() != 3 or k.dim() != 3 or tuple(q.shape) != (n, H, D) or k.shape != v.shape or k.shape[0] != n or k.shape[2] != D:
+        raise PttsError(ERR_ARG, f"expected q [{n}, {H}, {D}] and k, v [{n}, KVH, {D}]")
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not t.is_contiguous():
+            raise PttsError(ERR_ARG, f"{name} must be contiguous")
+        if t.device.type != "cuda" or t.device.index != kv.device:
+            raise PttsError(ERR_ARG, f"{name} must be on cuda:{kv.device}, where the cache is")
+    if out is None:
+        if out_dtype not in _DTYPES:
+            raise PttsError(ERR_ARG, f"unknown out_dtype {out_dtype}")
+        dtype = torch.bfloat16 if _DTYPES[out_dtype] == BF16 else torch.float32
+        if stream is None:
+            out = torch.empty((n, H * D), dtype=dtype, device=q.device)
+        else:  # memory of the stream that writes it
+            with torch.cuda.stream(stream):
+                out = torch.empty((n, H * D), dtype=dtype, device=q.device)
+    elif tuple(out.shape) != (n, H * D) or not out.is_contiguous() or out.device != q.device:
+        raise PttsError(ERR_ARG, f"out must be a contiguous [{n}, {H * D}] on cuda:{kv.device}")
+    rules = Scores(softcap, _rule_tensor(kv, slopes, "slopes", torch.float32, H),
+                   _rule_tensor(kv, first, "first", torch.int32, n), _rule_tensor(kv, last, "last", torch.int32, n))
+    args = (kv.handle, layer, q.data_ptr(), k.data_ptr(), v.data_ptr(), code, int(k.shape[1]), _ip(s), _ip(r), len(s))
+    tail = (max_period, ctypes.byref(rules), out.data_ptr(), _dtype_code(out), _stream_of(kv.device, stream))
+    if tree:
+        if parents is None:
+            raise PttsError(ERR_ARG, "parents are missing")
+        _check(lib().ptts_b200_attend_tree(*args, _rule_tensor(kv, parents, "parents", torch.int32, n), *tail))
+    else:
+        _check(lib().ptts_b200_attend_scored(*args, *tail))
+    return out
+
+
+def attend_scored(kv: KvState, layer: int, q, k, v, streams: Sequence[int], rows: Sequence[int], *,
+                  softcap: float = 0.0, slopes=None, first=None, last=None, max_period: float = 10000.0,
+                  out_dtype: str = "f32", out=None, stream=None):
+    """attend with score rules (see ptts_b200_attend_scored): scores capped by softcap * tanh(s /
+    softcap), biased by -slopes[head] * |position - key position| (slopes f32 [H]), each row seeing
+    the positions first..last (int32 [n_rows]; None: 0 and its own position). All on the cache's
+    device. max_period 0: no rotation. A row that sees nothing is zeros.
+
+    Masks as spans, for a row at position p: documents packed in one stream, first = the start of
+    p's document; a prefix that sees itself whole, last = max(p, prefix - 1); a window of w,
+    first = p - w + 1; a padding row, first > last."""
+    return _attend_rules(kv, layer, q, k, v, streams, rows, None, False, softcap, slopes, first, last, max_period,
+                         out_dtype, out, stream)
+
+
+def attend_tree(kv: KvState, layer: int, q, k, v, streams: Sequence[int], rows: Sequence[int], parents, *,
+                softcap: float = 0.0, slopes=None, first=None, max_period: float = 10000.0,
+                out_dtype: str = "f32", out=None, stream=None):
+    """Attention of drafted trees over the cache (see ptts_b200_attend_tree): rows[i] nodes (at most
+    64) on stream streams[i]; parents int32 [n_rows], a node's parent within its sequence (below its
+    own index) or -1. A node sees the cached rows, its ancestors and itself, at position length +
+    depth; its k and v go to slot length + index. KvState.accept keeps a path."""
+    return _attend_rules(kv, layer, q, k, v, streams, rows, parents, True, softcap, slopes, first, None, max_period,
+                         out_dtype, out, stream)
 
 
 def step_lanes(n: int) -> int:

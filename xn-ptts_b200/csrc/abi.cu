@@ -15,6 +15,7 @@
 #include "host.h"
 #include "kernels.h"
 #include "ptts_b200.h"
+#include "score.h"
 
 uint64_t ptts_b200_flow_prepare(ptts_b200_flow* f, int n, int d_model);
 int ptts_b200_flow_ldim(const ptts_b200_flow* f);
@@ -179,6 +180,8 @@ struct ptts_b200_kv {
     std::vector<int32_t> h_window;
     // scratch of the attention op
     DevBuf seq_stream, row_offsets, row_stream, row_pos, prefix, part, q_rot, counters;
+    // scratch of the scored and tree attention: the rows' plan, their lineages, the work units
+    DevBuf score_rows, lineage, units;
     Staging staging;
     // What seq_stream holds after the last upload_seq, and on which CUDA stream it was copied: a
     // decode loop that attends and advances the same streams step after step copies the list
@@ -566,6 +569,110 @@ void check_model_kv(const ptts_b200_model* m, const ptts_b200_kv* kv) {
     for (int l = 0; l < m->cfg.num_layers; ++l)
         require(m->layers[l]->loaded, PTTS_B200_ERR_STATE,
                 "layer " + std::to_string(l) + " has no weights (ptts_b200_model_load_layer)");
+}
+
+// The calls below plan from the host's lengths, so a replay of a captured call would use old ones.
+void refuse_capture(cudaStream_t s, const char* what) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    CK(cudaStreamIsCapturing(s, &st));
+    if (st != cudaStreamCaptureStatusNone)
+        fail(PTTS_B200_ERR_STATE, std::string(what) + " plans from the host's lengths: it cannot be captured in a CUDA graph");
+}
+
+// The scored attention of prompts and single tokens (parents nullptr) and of drafted trees.
+void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* k, const void* v, int in_dtype,
+                        int num_kv_heads, const int32_t* streams_host, const int32_t* rows_host, int n_seq,
+                        const int32_t* parents, bool tree, float max_period, const ptts_b200_scores* scores, void* out,
+                        int out_dtype, cudaStream_t s) {
+    check_kv(kv);
+    require(layer >= 0 && layer < kv->layers, PTTS_B200_ERR_ARG, "layer out of range");
+    require(q && k && v && out, PTTS_B200_ERR_ARG, "q/k/v/out are NULL");
+    require(in_dtype == PTTS_B200_F32 || in_dtype == PTTS_B200_BF16, PTTS_B200_ERR_ARG, "bad in_dtype");
+    require(out_dtype == PTTS_B200_F32 || out_dtype == PTTS_B200_BF16, PTTS_B200_ERR_ARG, "bad out_dtype");
+    if (num_kv_heads <= 0 || kv->heads % num_kv_heads != 0)
+        fail(PTTS_B200_ERR_ARG, "the " + std::to_string(num_kv_heads) + " key/value heads do not divide the " +
+                                    std::to_string(kv->heads) + " attention heads");
+    require(max_period == 0.0f || (max_period > 1.0f && std::isfinite(max_period)), PTTS_B200_ERR_ARG,
+            "max_period must be above 1, or 0 for no rotation");
+    const ptts_b200_scores none{};
+    const ptts_b200_scores& sc = scores ? *scores : none;
+    require(sc.softcap >= 0.0f && std::isfinite(sc.softcap), PTTS_B200_ERR_ARG, "softcap must be 0 (none) or positive");
+    auto aligned = [](const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
+    require(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16), PTTS_B200_ERR_ARG,
+            "q, k, v and out must be aligned to 16 bytes");
+    require(aligned(sc.slopes, 4) && aligned(sc.first, 4) && aligned(sc.last, 4) && aligned(parents, 4),
+            PTTS_B200_ERR_ARG, "slopes, first, last and parents must be aligned to 4 bytes");
+    std::vector<int32_t> offsets;
+    const int n_rows = check_sequences(kv, streams_host, rows_host, n_seq, offsets);
+    for (int i = 0; i < n_seq; ++i)
+        if (kv->is_ring(streams_host[i]) || kv->is_window(streams_host[i]))
+            fail(PTTS_B200_ERR_UNSUPPORTED, "stream " + std::to_string(streams_host[i]) +
+                                                " is a ring or windowed: score rules and trees run on appended streams");
+    if (tree) {
+        require(parents != nullptr, PTTS_B200_ERR_ARG, "parents are NULL");
+        require(sc.last == nullptr, PTTS_B200_ERR_ARG, "a drafted node sees up to itself: last must be NULL");
+        for (int i = 0; i < n_seq; ++i)
+            if (rows_host[i] > kTreeNodes)
+                fail(PTTS_B200_ERR_UNSUPPORTED, "a tree has at most " + std::to_string(kTreeNodes) + " nodes, not " +
+                                                    std::to_string(rows_host[i]));
+    }
+    DeviceScope scope(kv->device);
+    refuse_capture(s, tree ? "ptts_b200_attend_tree" : "ptts_b200_attend_scored");
+    const bool cache_bf16 = kv->dtype == PTTS_B200_BF16;
+    const size_t hd = (size_t)kv->heads * kHeadDim;
+    std::vector<int32_t> packed(streams_host, streams_host + n_seq);
+    packed.insert(packed.end(), offsets.begin(), offsets.end());
+    const int32_t* d = kv->upload_seq(packed, s);
+    ScorePlanArgs p{};
+    p.seq_stream = d;
+    p.row_offsets = d + n_seq;
+    p.n_seq = n_seq;
+    p.n_rows = n_rows;
+    p.lengths = kv->len.as<int32_t>();
+    p.num_streams = kv->streams;
+    p.capacity = kv->capacity;
+    p.parents = tree ? parents : nullptr;
+    p.first = sc.first;
+    p.last = sc.last;
+    p.q = q;
+    p.k = k;
+    p.v = v;
+    p.q_out = static_cast<float*>(kv->q_rot.need((size_t)n_rows * hd * sizeof(float)));
+    p.k_cache = kv->k_layer(layer);
+    p.v_cache = kv->v_layer(layer);
+    p.heads = kv->heads;
+    p.kv_heads = num_kv_heads;
+    p.rotate = max_period != 0.0f;
+    if (p.rotate) rope_inv_freq(kv->head_dim, max_period, p.inv_freq);
+    int32_t* rows = static_cast<int32_t*>(kv->score_rows.need(sizeof(int32_t) * (tree ? 6 : 4) * (size_t)n_rows));
+    p.rows.stream = rows;
+    p.rows.pos = rows + n_rows;
+    p.rows.lo = rows + 2 * (size_t)n_rows;
+    p.rows.hi = rows + 3 * (size_t)n_rows;
+    if (tree) {
+        p.rows.base = rows + 4 * (size_t)n_rows;
+        p.rows.row0 = rows + 5 * (size_t)n_rows;
+        p.rows.lineage = static_cast<unsigned long long*>(kv->lineage.need(sizeof(unsigned long long) * n_rows));
+    }
+    p.err = kv->err.as<uint32_t>();
+    launch_score_plan(p, in_dtype == PTTS_B200_BF16, cache_bf16, s);
+    check_launch();
+    ScoreCoreArgs a{};
+    a.k_cache = p.k_cache;
+    a.v_cache = p.v_cache;
+    a.q = p.q_out;
+    a.out = out;
+    a.out_bf16 = out_dtype == PTTS_B200_BF16;
+    a.n_rows = n_rows;
+    a.heads = kv->heads;
+    a.num_streams = kv->streams;
+    a.capacity = kv->capacity;
+    a.rows = p.rows;
+    a.rule.cap = sc.softcap;
+    a.rule.slopes = sc.slopes;
+    a.err = p.err;
+    launch_score_core(a, cache_bf16, s);
+    check_launch();
 }
 
 // Split-K slices of out_proj and linear2 at a row count: enough CTAs to fill the GPU at decode
@@ -1417,6 +1524,95 @@ int ptts_b200_attend(ptts_b200_kv* kv, int layer, const void* q, const void* k, 
             bytes += (double)n_seq * hd * (4 + (out_dtype == PTTS_B200_BF16 ? 2 : 4));
             trace_add(1, ms, bytes, 0, 0.0);
         }
+    });
+}
+
+int ptts_b200_attend_scored(ptts_b200_kv* kv, int layer, const void* q, const void* k, const void* v,
+                            int in_dtype, int num_kv_heads, const int32_t* streams_host,
+                            const int32_t* rows_host, int n_seq, float max_period,
+                            const ptts_b200_scores* scores, void* out, int out_dtype, void* cuda_stream) {
+    return guarded([&] {
+        attend_with_scores(kv, layer, q, k, v, in_dtype, num_kv_heads, streams_host, rows_host, n_seq, nullptr, false,
+                           max_period, scores, out, out_dtype, as_stream(cuda_stream));
+    });
+}
+
+int ptts_b200_attend_tree(ptts_b200_kv* kv, int layer, const void* q, const void* k, const void* v,
+                          int in_dtype, int num_kv_heads, const int32_t* streams_host,
+                          const int32_t* rows_host, int n_seq, const int32_t* parents, float max_period,
+                          const ptts_b200_scores* scores, void* out, int out_dtype, void* cuda_stream) {
+    return guarded([&] {
+        attend_with_scores(kv, layer, q, k, v, in_dtype, num_kv_heads, streams_host, rows_host, n_seq, parents, true,
+                           max_period, scores, out, out_dtype, as_stream(cuda_stream));
+    });
+}
+
+int ptts_b200_kv_accept(ptts_b200_kv* kv, const int32_t* streams_host, const int32_t* counts_host,
+                        const int32_t* nodes_host, int n, void* cuda_stream) {
+    return guarded([&] {
+        check_kv(kv);
+        require(n > 0, PTTS_B200_ERR_ARG, "n must be positive");
+        require(streams_host && counts_host, PTTS_B200_ERR_ARG, "streams/counts are NULL");
+        std::vector<char> seen(kv->streams, 0);
+        std::vector<int32_t> list(3 * (size_t)n + 1);
+        int32_t *lens = list.data() + n, *offsets = list.data() + 2 * (size_t)n;
+        long long total = 0;
+        for (int i = 0; i < n; ++i) {
+            const int st = streams_host[i], c = counts_host[i];
+            if (st < 0 || st >= kv->streams)
+                fail(PTTS_B200_ERR_ARG,
+                     "stream " + std::to_string(st) + " is outside 0.." + std::to_string(kv->streams - 1));
+            if (seen[st]) fail(PTTS_B200_ERR_ARG, "stream " + std::to_string(st) + " appears twice");
+            seen[st] = 1;
+            if (kv->is_ring(st) || kv->is_window(st))
+                fail(PTTS_B200_ERR_UNSUPPORTED, "stream " + std::to_string(st) +
+                                                    " is a ring or windowed: score rules and trees run on appended streams");
+            if (c < 0 || c > kTreeNodes)
+                fail(PTTS_B200_ERR_ARG, "an accepted path has 0.." + std::to_string(kTreeNodes) + " nodes, not " +
+                                            std::to_string(c));
+            require(c == 0 || nodes_host, PTTS_B200_ERR_ARG, "nodes are NULL");
+            for (int j = 0; j < c; ++j) {
+                const int x = nodes_host[total + j];
+                if (x < (j ? nodes_host[total + j - 1] + 1 : 0) || x >= kTreeNodes)
+                    fail(PTTS_B200_ERR_ARG, "an accepted path's nodes rise within 0.." + std::to_string(kTreeNodes - 1) +
+                                                " (stream " + std::to_string(st) + ")");
+            }
+            if (c && (long long)kv->h_len[st] + nodes_host[total + c - 1] >= kv->capacity)
+                fail(PTTS_B200_ERR_CAPACITY, "node " + std::to_string(nodes_host[total + c - 1]) + " past " +
+                                                 std::to_string(kv->h_len[st]) +
+                                                 " filled KV positions is outside a budget of " +
+                                                 std::to_string(kv->capacity) + " (stream " + std::to_string(st) + ")");
+            list[i] = st;
+            lens[i] = kv->h_len[st];
+            offsets[i] = (int32_t)total;
+            total += c;
+        }
+        offsets[n] = (int32_t)total;
+        list.insert(list.end(), nodes_host, nodes_host + total);
+        DeviceScope scope(kv->device);
+        cudaStream_t s = as_stream(cuda_stream);
+        refuse_capture(s, "ptts_b200_kv_accept");
+        AcceptArgs a{};
+        a.k_cache = kv->k.p;
+        a.v_cache = kv->v.p;
+        a.block_vec = (long long)kv->group_bytes() / 16;
+        a.stream_vec = (long long)kv->stream_bytes() / 16;
+        a.row_vec = (int)kv->group_row_bytes() / 16;
+        a.blocks = kv->layers * kv->groups();
+        a.streams = kv->streams;
+        a.capacity = kv->capacity;
+        a.n = n;
+        a.lengths = kv->len.as<int32_t>();
+        a.err = kv->err.as<uint32_t>();
+        if (list.size() <= (size_t)kAcceptInline) {
+            AcceptInline in;
+            std::copy(list.begin(), list.end(), in.list);
+            launch_accept_inline(a, in, s);
+        } else {
+            launch_accept(a, kv->upload_scratch(list.data(), sizeof(int32_t) * list.size(), s), s);
+        }
+        check_launch();
+        for (int i = 0; i < n; ++i) kv->h_len[streams_host[i]] += counts_host[i];
     });
 }
 

@@ -1,0 +1,108 @@
+// Internal launchers of attention with score rules (softcap, distance bias, spans) and of drafted
+// trees: the row plan, the kernels that read it, and the acceptance of a drafted path.
+//
+// A row at position p of a stream sees cache slots lo..hi (slot = position); in a tree call the
+// slots from `base` (the stream's length) on hold the drafted nodes, of which a row sees those in
+// its lineage: bit i = node i. With s_j = q . k_j / 8 over the visible slots j:
+//   t_j = cap * tanh(s_j / cap)             (s_j where cap is 0)
+//   u_j = t_j - slopes[h] * |p - pos(j)|    (t_j without slopes; pos(j) = j, or a node's position)
+//   out = sum_j exp(u_j) v_j / sum_j exp(u_j), zeros where nothing is visible.
+#pragma once
+
+#include "kernels.h"
+
+namespace ptts {
+
+constexpr int kTreeNodes = 64;  // drafted nodes per stream: one bit each
+
+// Per row, on the device (written by the plan).
+struct ScoreRows {
+    int32_t* stream = nullptr;  // arena stream; -1: the plan refused the row (it sees nothing)
+    int32_t* pos = nullptr;     // RoPE position, and the p of the distance bias
+    int32_t* lo = nullptr;      // first visible slot
+    int32_t* hi = nullptr;      // last visible slot; lo > hi: the row sees nothing
+    int32_t* base = nullptr;    // tree calls: the stream's cached length
+    int32_t* row0 = nullptr;    // tree calls: the row of the stream's node 0
+    unsigned long long* lineage = nullptr;  // tree calls: nodes the row sees, itself among them; else nullptr
+};
+
+struct ScoreRule {
+    float cap = 0.f;                // 0: none
+    const float* slopes = nullptr;  // [H] or nullptr
+};
+
+struct ScorePlanArgs {
+    // What the host sends: streams [n_seq], row offsets [n_seq + 1].
+    const int32_t* seq_stream;
+    const int32_t* row_offsets;
+    int n_seq, n_rows;
+    const int32_t* lengths;   // [num_streams]
+    int num_streams, capacity;
+    const int32_t* parents;   // [n_rows] tree calls, else nullptr
+    const int32_t* first;     // [n_rows] or nullptr
+    const int32_t* last;      // [n_rows] or nullptr (spans only)
+    // RoPE (unless !rotate) and append, as RopeAppendArgs.
+    const void* q;
+    const void* k;
+    const void* v;
+    float* q_out;                   // [n_rows][H * 64] f32, rotated, or nullptr:
+    __nv_bfloat16* q_hi = nullptr;  // q * q_scale as bf16 hi and lo planes
+    __nv_bfloat16* q_lo = nullptr;
+    float q_scale = 1.f;
+    void* k_cache;
+    void* v_cache;
+    int heads, kv_heads;
+    bool rotate;
+    float inv_freq[kMaxPairs];
+    ScoreRows rows;
+    // Split kernels: the work units (single rows, or blocks of consecutive rows of one sequence:
+    // (first row, rows)), their key counts laid end to end, and the unit each CTA starts in.
+    const int2* blocks = nullptr;  // [n_units]; nullptr: unit u is row u
+    int n_units = 0;               // 0: no units
+    int32_t* prefix = nullptr;     // [n_units + 1]
+    int32_t* unit_lo = nullptr;    // [n_units] first slot any row of the unit sees
+    int32_t* cta_first = nullptr;  // [grid]
+    int grid = 0;
+    uint32_t* err;
+};
+// One launch: every row's plan entry, its rotated q, its cache rows; and the units' partition.
+void launch_score_plan(const ScorePlanArgs& a, bool in_bf16, bool cache_bf16, cudaStream_t s);
+
+// Attention on CUDA cores, one warp per (row, head), any cache type.
+struct ScoreCoreArgs {
+    const void* k_cache;  // the layer: kv_offset's layout
+    const void* v_cache;
+    const float* q;       // [n_rows][H * 64] f32, rotated
+    void* out;            // [n_rows][H * 64]
+    bool out_bf16;
+    int n_rows, heads, num_streams, capacity;
+    ScoreRows rows;
+    ScoreRule rule;
+    uint32_t* err;
+};
+void launch_score_core(const ScoreCoreArgs& a, bool cache_bf16, cudaStream_t s);
+
+// Acceptance: per stream the accepted nodes' rows move from slot len + node[j] to len + j, in
+// every layer and head group, and the length becomes len + their number. Nodes rise, so
+// node[j] >= j. The lists are one array of int32 (host or device): streams [n], lengths before
+// [n], offsets into the nodes [n + 1], nodes.
+constexpr int kAcceptInline = 512;
+struct AcceptInline {  // a short list rides in the launch's parameters
+    int32_t list[kAcceptInline];
+};
+struct AcceptArgs {
+    void* k_cache;         // all layers
+    void* v_cache;
+    long long block_vec;   // 16-byte vectors of one (layer, group) block
+    long long stream_vec;  // of one stream in a block
+    int row_vec;           // of one row of a group
+    int blocks;            // layers * groups
+    int streams, capacity;
+    int n;
+    int32_t* lengths;
+    uint32_t* err;
+};
+void launch_accept(const AcceptArgs& a, const int32_t* list_dev, cudaStream_t s);
+void launch_accept_inline(const AcceptArgs& a, const AcceptInline& list, cudaStream_t s);
+
+}  // namespace ptts
