@@ -655,8 +655,50 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
         p.rows.lineage = static_cast<unsigned long long*>(kv->lineage.need(sizeof(unsigned long long) * n_rows));
     }
     p.err = kv->err.as<uint32_t>();
+    // Single tokens run on the split-KV decode, a row per unit.
+    const bool tokens = !tree && n_rows == n_seq;
+    const int grid = sm_count(kv->device);
+    if (tokens) {
+        p.n_units = n_rows;
+        p.grid = grid;
+        p.prefix = static_cast<int32_t*>(kv->units.need(sizeof(int32_t) * (2 * (size_t)p.n_units + 1 + grid)));
+        p.unit_lo = p.prefix + p.n_units + 1;
+        p.cta_first = p.unit_lo + p.n_units;
+    }
     launch_score_plan(p, in_dtype == PTTS_B200_BF16, cache_bf16, s);
     check_launch();
+    if (tokens) {
+        const size_t n_part = decode_part_floats(n_rows, grid), n_cnt = decode_counter_ints(n_rows);
+        const size_t out_elem = out_dtype == PTTS_B200_BF16 ? 2 : 4;
+        for (int g = 0; g < kv->groups(); ++g) {
+            const size_t col = (size_t)g * kRowWidth;
+            DecodeArgs a{};
+            a.k_cache = kv->k_group(layer, g);
+            a.v_cache = kv->v_group(layer, g);
+            a.stream_bytes = (long long)kv->stream_bytes();
+            a.row_stream = p.rows.stream;
+            a.row_pos = p.rows.pos;
+            a.row_lo = p.rows.lo;
+            a.row_hi = p.rows.hi;
+            a.unit_lo = p.unit_lo;
+            a.prefix = p.prefix;
+            a.cta_first = p.cta_first;
+            a.q = p.q_out + col;
+            a.out = static_cast<char*>(out) + col * out_elem;
+            a.out_mode = out_dtype == PTTS_B200_BF16 ? kOutBf16 : kOutF32;
+            a.ld = (int)hd;
+            a.part = static_cast<float*>(kv->part.need(sizeof(float) * n_part * kv->groups())) + n_part * g;
+            a.counters = static_cast<int*>(kv->counters.need_zeroed(sizeof(int) * n_cnt * kv->groups())) + n_cnt * g;
+            a.B = n_rows;
+            a.capacity = kv->capacity;
+            a.cap = sc.softcap;
+            a.slopes = sc.slopes ? sc.slopes + g * kGroupHeads : nullptr;
+            a.err = p.err;
+            launch_decode_attn_scored(a, cache_bf16, grid, s);
+            check_launch();
+        }
+        return;
+    }
     ScoreCoreArgs a{};
     a.k_cache = p.k_cache;
     a.v_cache = p.v_cache;

@@ -28,8 +28,13 @@
 // 128-byte slice of every row with 16-byte shared loads (8 lanes per row, 4 rows per warp
 // instruction) and keep an online softmax in the exp2 domain. Every wait is bounded and reports
 // DEV_ERR_TIMEOUT.
+//
+// With score rules (SCORED): the same split and ring over each row's visible span, its scores capped
+// and biased in f32 between the dot product and the running maximum (see score.h). The rules cost
+// issue slots the copies leave idle: see the rates below the kernel
 #include "common.cuh"
 #include "kernels.h"
+#include "score.cuh"
 
 namespace ptts {
 namespace {
@@ -66,8 +71,10 @@ struct ChunkHdr {
     int sid;         // arena stream
     int ring_w;      // ring write slot, or -1
     int c0, c1;      // the CTAs holding pieces of a cut stream
+    int at;          // SCORED: the row's position less its first visible slot (key i is at - i away)
 };
 constexpr int kFirst = 1, kLast = 2, kWhole = 4, kEnd = 8;
+constexpr int kEmpty = 32;    // SCORED: the row sees nothing (its one counted key is not used)
 constexpr int kQLoaded = 16;  // the consumers loaded this piece's q themselves (none in the stage)
 
 template <typename T>
@@ -185,7 +192,7 @@ __device__ __forceinline__ void merge_head(const DecodeArgs& a, int b, int h, in
     }
 }
 
-template <typename T, class R>
+template <typename T, class R, bool SCORED = false>
 __global__ void __launch_bounds__(kThreads, 1) decode_attn_kernel(DecodeArgs a) {
     constexpr int kStages = R::kStages, kDataBytes = R::kDataBytes, kStageBytes = R::kStageBytes;
     constexpr int RB = Row<T>::kBytes;
@@ -259,16 +266,20 @@ __global__ void __launch_bounds__(kThreads, 1) decode_attn_kernel(DecodeArgs a) 
             const int s0 = (int)((start > pb ? start : pb) - pb);
             const int s1 = (int)((end < pe ? end : pe) - pb);
             const bool whole = pb >= start && pe <= end;
-            const int sid = a.row_stream[b];
+            const int sid = SCORED ? max(a.row_stream[b], 0) : a.row_stream[b];  // -1: refused, sees nothing
             const long long base = (long long)sid * a.stream_bytes;
             // Key i of the stream sits at slot i, or for a windowed stream at slot
             // (first + i) % capacity, first being the oldest attended position.
-            const bool wrap = a.window && a.capacity > 0 && a.window[sid] > 0;
-            const int first = wrap ? (int)(((long long)a.row_pos[b] + 1 - (pe - pb)) % a.capacity) : 0;
+            const bool wrap = !SCORED && a.window && a.capacity > 0 && a.window[sid] > 0;
+            const int first = SCORED ? a.unit_lo[b]
+                              : wrap ? (int)(((long long)a.row_pos[b] + 1 - (pe - pb)) % a.capacity)
+                                     : 0;
             ChunkHdr proto;
             proto.b = b;
             proto.sid = sid;
-            proto.ring_w = a.ring_write ? a.ring_write[sid] : -1;
+            proto.ring_w = !SCORED && a.ring_write ? a.ring_write[sid] : -1;
+            proto.at = SCORED ? a.row_pos[b] - first : 0;
+            const int empty = SCORED && a.row_lo[b] > a.row_hi[b] ? kEmpty : 0;
             proto.c0 = whole ? c : cta_of(pb, total, G);
             proto.c1 = whole ? c : cta_of(pe - 1, total, G);
             for (int p = s0; p < s1; p += CH, ++it) {
@@ -285,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_attn_kernel(DecodeArgs a) 
                 hd.n = n;
                 const bool q_loaded = it == 0 && q_first_loaded;  // the CTA's first chunk: stream b0
                 hd.flags = (p == s0 ? kFirst : 0) | (p + n >= s1 ? kLast : 0) | (whole ? kWhole : 0) |
-                           (q_loaded ? kQLoaded : 0);
+                           (q_loaded ? kQLoaded : 0) | empty;
                 *reinterpret_cast<ChunkHdr*>(sb + kDataBytes + kQStageBytes) = hd;
                 mbar_arrive_expect_tx(&full[st], 2u * n * RB + (p == s0 && !q_loaded ? (uint32_t)kQStageBytes : 0u));
                 if (p == s0 && !q_loaded) {
@@ -296,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_attn_kernel(DecodeArgs a) 
                         q_row[n_deferred++] = b;
                     }
                 }
-                const int slot = wrap ? (first + p) % a.capacity : p;
+                const int slot = SCORED ? first + p : wrap ? (first + p) % a.capacity : p;
                 const int n0 = wrap ? min(n, a.capacity - slot) : n;  // rows before the wrap
                 bulk_g2s(sb, kc + base + (long long)slot * RB, n0 * RB, &full[st], pol);
                 bulk_g2s(sb + kDataBytes / 2, vc + base + (long long)slot * RB, n0 * RB, &full[st], pol);
@@ -328,7 +339,10 @@ __global__ void __launch_bounds__(kThreads, 1) decode_attn_kernel(DecodeArgs a) 
     const int h = warp;
     const int g = lane >> 3;  // which of the 4 rows of a warp step
     const int j = lane & 7;   // which 16-byte slice of the head row
-    float q[8], m = -1e30f, l = 0.f, acc[8];
+    // Below every score of the plain op's inputs; a bias can carry scores further down.
+    constexpr float kLow = SCORED ? kScoreLow : -1e30f;
+    float q[8], m = kLow, l = 0.f, acc[8];
+    const float slope = SCORED && a.slopes ? a.slopes[h] : 0.f;
     // The q of the CTA's first piece (stream cta_first[c]), loaded now rather than staged.
     float q_first[8];
     if (a.prestart && a.cta_first) {
@@ -352,8 +366,8 @@ __global__ void __launch_bounds__(kThreads, 1) decode_attn_kernel(DecodeArgs a) 
                 load_q<T>(reinterpret_cast<const float*>(sb + kDataBytes) + h * kHeadDim, j, q);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] *= a.qscale;
-            m = -1e30f;
+            for (int i = 0; i < 8; ++i) q[i] *= SCORED ? 0.125f : a.qscale;
+            m = kLow;
             l = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) acc[i] = 0.f;
@@ -406,6 +420,10 @@ __global__ void __launch_bounds__(kThreads, 1) decode_attn_kernel(DecodeArgs a) 
                 d0 += __shfl_xor_sync(0xffffffffu, d0, o);
                 d1 += __shfl_xor_sync(0xffffffffu, d1, o);
             }
+            if constexpr (SCORED) {
+                d0 = score_exact(d0, a.cap, slope, hd.at - p - r0);
+                d1 = score_exact(d1, a.cap, slope, hd.at - p - r1);
+            }
             if (r0 >= n) d0 = -INFINITY;
             if (r1 >= n) d1 = -INFINITY;
             if (vis) {
@@ -455,6 +473,10 @@ __global__ void __launch_bounds__(kThreads, 1) decode_attn_kernel(DecodeArgs a) 
                 const float inv = 1.f / ll;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) aa[i] *= inv;
+                if (SCORED && (hd.flags & kEmpty)) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) aa[i] = 0.f;
+                }
                 store_out<T>(a, (long long)b * a.ld + h * kHeadDim, j, aa);
             }
             continue;
@@ -486,10 +508,10 @@ __global__ void __launch_bounds__(kThreads, 1) decode_attn_kernel(DecodeArgs a) 
     if (lane == 0) stamp_mark(a.stamps, a.stamp, STAMP_END);
 }
 
-template <typename T, class R>
+template <typename T, class R, bool SCORED = false>
 void launch_typed(const DecodeArgs& a, int grid, cudaStream_t s) {
-    set_max_dynamic_smem(reinterpret_cast<const void*>(decode_attn_kernel<T, R>), R::kSmemBytes);
-    launch_k(decode_attn_kernel<T, R>, dim3(grid), dim3(kThreads), R::kSmemBytes, s, a);
+    set_max_dynamic_smem(reinterpret_cast<const void*>(decode_attn_kernel<T, R, SCORED>), R::kSmemBytes);
+    launch_k(decode_attn_kernel<T, R, SCORED>, dim3(grid), dim3(kThreads), R::kSmemBytes, s, a);
 }
 
 }  // namespace
@@ -508,6 +530,11 @@ void launch_decode_attn(const DecodeArgs& a, bool cache_bf16, int grid, cudaStre
         if (cache_bf16) launch_typed<__nv_bfloat16, WideRing>(a, grid, s);
         else launch_typed<float, WideRing>(a, grid, s);
     }
+}
+
+void launch_decode_attn_scored(const DecodeArgs& a, bool cache_bf16, int grid, cudaStream_t s) {
+    if (cache_bf16) launch_typed<__nv_bfloat16, WideRing, true>(a, grid, s);
+    else launch_typed<float, WideRing, true>(a, grid, s);
 }
 
 }  // namespace ptts

@@ -226,6 +226,15 @@ struct DecodeArgs {
     // before that predecessor began (it is not the plan kernel): the kernel reads the plan and
     // copies those rows before it waits for the predecessor.
     bool prestart = false;
+    // launch_decode_attn_scored only (never with prestart, rings or windows): row b's keys are the
+    // slots unit_lo[b] on, none of them visible when row_lo[b] > row_hi[b] (one key is counted all
+    // the same, so that its zeros are written); score rules as in score.h, slopes of this launch's
+    // 8 heads. q is scaled by 1 / sqrt(D) in the kernel; qscale is not read.
+    const int32_t* unit_lo = nullptr;
+    const int32_t* row_lo = nullptr;
+    const int32_t* row_hi = nullptr;
+    float cap = 0.f;
+    const float* slopes = nullptr;
 };
 // Output forms of the attention kernels.
 constexpr int kOutF32 = 0, kOutBf16 = 1, kOutHiLo = 2;  // hi/lo: f16(o) and f16(o - hi)
@@ -234,6 +243,8 @@ constexpr int kPartStride = 68;  // floats per (slot, head) partial: acc[64], m,
 // than one CTA are merged by the CTA that finishes them last. `grid` CTAs at most (one per SM).
 // `compact`: the smaller shared-memory ring, which leaves room on each SM for a linear's CTA.
 void launch_decode_attn(const DecodeArgs& a, bool cache_bf16, int grid, cudaStream_t s, bool compact = false);
+// The same with score rules and visible spans (the wide ring).
+void launch_decode_attn_scored(const DecodeArgs& a, bool cache_bf16, int grid, cudaStream_t s);
 size_t decode_part_floats(int B, int grid);
 size_t decode_counter_ints(int B);
 

@@ -18,8 +18,10 @@ constexpr int kPlanThreads = 256;
 constexpr int kPlanWarps = kPlanThreads / 32;
 
 // The last sequence whose rows begin at or before row r.
-__device__ __forceinline__ int seq_of(const int32_t* __restrict__ offsets, int n_seq, int r) {
-    int lo = 0, hi = n_seq - 1;
+__device__ __forceinline__ int seq_of(const ScorePlanArgs& a, int r) {
+    if (a.n_seq == a.n_rows) return r;  // single tokens
+    const int32_t* offsets = a.row_offsets;
+    int lo = 0, hi = a.n_seq - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (offsets[mid] <= r) lo = mid;
@@ -52,7 +54,7 @@ __device__ void plan_units(const ScorePlanArgs& a) {
     if (a.blocks && spans) {
         for (int u = warp; u < a.n_units; u += kPlanWarps) {
             const int2 b = a.blocks[u];
-            const int sq = seq_of(a.row_offsets, a.n_seq, b.x), row0 = a.row_offsets[sq];
+            const int sq = seq_of(a, b.x), row0 = a.row_offsets[sq];
             const int base = a.lengths[a.seq_stream[sq]], rows = a.row_offsets[sq + 1] - row0;
             int lo = 0x7fffffff, hi = -1;
             for (int i = lane; i < b.y; i += 32) {
@@ -80,7 +82,7 @@ __device__ void plan_units(const ScorePlanArgs& a) {
                 v = a.prefix[u + 1];
             } else {
                 const int2 b = a.blocks ? a.blocks[u] : make_int2(u, 1);
-                const int sq = seq_of(a.row_offsets, a.n_seq, b.x), row0 = a.row_offsets[sq];
+                const int sq = seq_of(a, b.x), row0 = a.row_offsets[sq];
                 const int base = a.lengths[a.seq_stream[sq]], rows = a.row_offsets[sq + 1] - row0;
                 int lo, hi;
                 row_span(a, b.x + b.y - 1, base, row0, rows, lo, hi);  // without spans the last row sees the most
@@ -143,7 +145,7 @@ __global__ void __launch_bounds__(kPlanThreads) score_plan_kernel(ScorePlanArgs 
         }
         r -= 1;
     }
-    const int sq = seq_of(a.row_offsets, a.n_seq, r), row0 = a.row_offsets[sq];
+    const int sq = seq_of(a, r), row0 = a.row_offsets[sq];
     const int rows = a.row_offsets[sq + 1] - row0, sid = a.seq_stream[sq];
     const bool known = sid >= 0 && sid < a.num_streams;
     const int base = known ? a.lengths[sid] : 0;
