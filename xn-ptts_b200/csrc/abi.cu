@@ -620,8 +620,21 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
     refuse_capture(s, tree ? "ptts_b200_attend_tree" : "ptts_b200_attend_scored");
     const bool cache_bf16 = kv->dtype == PTTS_B200_BF16;
     const size_t hd = (size_t)kv->heads * kHeadDim;
+    // Single tokens run on the split-KV decode, a row per unit; other calls on a bf16 cache in blocks
+    // of rows, split over the keys.
+    const bool tokens = !tree && n_rows == n_seq, few = !tokens && cache_bf16, out_bf16 = out_dtype == PTTS_B200_BF16;
+    int block = 0, grid = sm_count(kv->device);
+    std::vector<int2> blocks;
+    if (few) {
+        block = score_rows_block(*std::max_element(rows_host, rows_host + n_seq));
+        grid = score_rows_grid(block, kv->heads, grid);
+        for (int i = 0; i < n_seq; ++i)
+            for (int r = offsets[i]; r < offsets[i + 1]; r += block)
+                blocks.push_back(make_int2(r, std::min(block, offsets[i + 1] - r)));
+    }
     std::vector<int32_t> packed(streams_host, streams_host + n_seq);
     packed.insert(packed.end(), offsets.begin(), offsets.end());
+    const size_t blocks_at = append_tiles(packed, blocks);
     const int32_t* d = kv->upload_seq(packed, s);
     ScorePlanArgs p{};
     p.seq_stream = d;
@@ -655,15 +668,18 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
         p.rows.lineage = static_cast<unsigned long long*>(kv->lineage.need(sizeof(unsigned long long) * n_rows));
     }
     p.err = kv->err.as<uint32_t>();
-    // Single tokens run on the split-KV decode, a row per unit.
-    const bool tokens = !tree && n_rows == n_seq;
-    const int grid = sm_count(kv->device);
-    if (tokens) {
-        p.n_units = n_rows;
+    if (tokens || few) {
+        p.n_units = few ? (int)blocks.size() : n_rows;
+        p.blocks = few ? reinterpret_cast<const int2*>(d + blocks_at) : nullptr;
         p.grid = grid;
         p.prefix = static_cast<int32_t*>(kv->units.need(sizeof(int32_t) * (2 * (size_t)p.n_units + 1 + grid)));
         p.unit_lo = p.prefix + p.n_units + 1;
         p.cta_first = p.unit_lo + p.n_units;
+    }
+    if (few) {  // two bf16 planes in the f32 buffer
+        p.q_hi = reinterpret_cast<__nv_bfloat16*>(p.q_out);
+        p.q_lo = p.q_hi + (size_t)n_rows * hd;
+        p.q_scale = score_q_scale(sc.softcap, !out_bf16);
     }
     launch_score_plan(p, in_dtype == PTTS_B200_BF16, cache_bf16, s);
     check_launch();
@@ -697,6 +713,33 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
             launch_decode_attn_scored(a, cache_bf16, grid, s);
             check_launch();
         }
+        return;
+    }
+    if (few) {
+        ScoreRowsArgs a{};
+        a.k_cache = p.k_cache;
+        a.v_cache = p.v_cache;
+        a.q_hi = p.q_hi;
+        a.q_lo = p.q_lo;
+        a.out = out;
+        a.out_bf16 = out_bf16;
+        a.ld = (int)hd;
+        a.heads = kv->heads;
+        a.num_streams = kv->streams;
+        a.capacity = kv->capacity;
+        a.rows = p.rows;
+        a.rule.cap = sc.softcap;
+        a.rule.slopes = sc.slopes;
+        a.blocks = p.blocks;
+        a.n_units = p.n_units;
+        a.prefix = p.prefix;
+        a.unit_lo = p.unit_lo;
+        a.cta_first = p.cta_first;
+        a.part = static_cast<float*>(kv->part.need(sizeof(float) * score_rows_part_floats(block, kv->heads, grid)));
+        a.err = p.err;
+        require(launch_score_rows(a, block, grid, s), PTTS_B200_ERR_CUDA,
+                "could not describe the cache's tensors (cuTensorMapEncodeTiled)");
+        check_launch();
         return;
     }
     ScoreCoreArgs a{};

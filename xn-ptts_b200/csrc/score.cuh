@@ -21,4 +21,19 @@ __device__ __forceinline__ float score_exact(float s, float cap, float slope, in
     return (s - slope * (float)abs(distance)) * kScoreLog2e;
 }
 
+// The same in the exp2 domain, for scores out of the matrix products. Exact: x = s log2(e), by tanhf.
+__device__ __forceinline__ float cap_exact(float x, float cap) {
+    const float c = cap * kScoreLog2e;
+    return c * tanhf(x / c);
+}
+// Fast: x = 2 s log2(e) / cap, and tanh(y) = 1 - 2 / (1 + e^2y) by one exp2 and one reciprocal. Near
+// y = 0 the difference cancels: an absolute error of about cap x 2^-20, which moves a weight by at
+// most 2^-13 for cap <= kScoreFastCap, below bf16's own 2^-9.
+__device__ __forceinline__ float cap_fast(float x, float cap) {
+    const float c = cap * kScoreLog2e;
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + score_exp2(x)));
+    return fmaf(-2.f * c, r, c);
+}
+
 }  // namespace ptts

@@ -82,6 +82,45 @@ struct ScoreCoreArgs {
 };
 void launch_score_core(const ScoreCoreArgs& a, bool cache_bf16, cudaStream_t s);
 
+// How the matrix-product kernels cap scores: not, by the fast form (bf16 outputs, caps up to
+// kScoreFastCap; q is then scaled by 2 log2(e) / (8 cap)) or by tanhf (q scaled by log2(e) / 8, as
+// without a cap).
+enum { kCapNone = 0, kCapFast = 1, kCapExact = 2 };
+constexpr float kScoreFastCap = 128.f;
+inline int score_cap_mode(float cap, bool out_f32) {
+    return cap == 0.f ? kCapNone : (!out_f32 && cap <= kScoreFastCap ? kCapFast : kCapExact);
+}
+inline float score_q_scale(float cap, bool out_f32) {
+    constexpr float log2e = 1.4426950408889634f;
+    return score_cap_mode(cap, out_f32) == kCapFast ? 0.25f * log2e / cap : 0.125f * log2e;
+}
+
+// Few rows over a whole cache on mma.sync, bf16 caches (attn_rows.cu): blocks of up to
+// score_rows_block(most rows of a sequence) rows, the plan's units. False: the tensor maps could
+// not be made, nothing launched.
+struct ScoreRowsArgs {
+    const void* k_cache;  // the layer
+    const void* v_cache;
+    const __nv_bfloat16* q_hi;  // [n_rows][ld], scaled by score_q_scale
+    const __nv_bfloat16* q_lo;
+    void* out;            // [n_rows][ld]
+    bool out_bf16;
+    int ld, heads, num_streams, capacity;
+    ScoreRows rows;
+    ScoreRule rule;
+    const int2* blocks;   // [n_units]
+    int n_units;
+    const int32_t* prefix;
+    const int32_t* unit_lo;
+    const int32_t* cta_first;
+    float* part;          // score_rows_part_floats
+    uint32_t* err;
+};
+int score_rows_block(int most_rows);
+int score_rows_grid(int block, int heads, int sms);  // CTAs along the keys (the plan's grid)
+size_t score_rows_part_floats(int block, int heads, int grid);
+bool launch_score_rows(const ScoreRowsArgs& a, int block, int grid, cudaStream_t s);
+
 // Acceptance: per stream the accepted nodes' rows move from slot len + node[j] to len + j, in
 // every layer and head group, and the length becomes len + their number. Nodes rise, so
 // node[j] >= j. The lists are one array of int32 (host or device): streams [n], lengths before
