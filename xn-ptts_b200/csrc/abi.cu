@@ -620,13 +620,16 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
     refuse_capture(s, tree ? "ptts_b200_attend_tree" : "ptts_b200_attend_scored");
     const bool cache_bf16 = kv->dtype == PTTS_B200_BF16;
     const size_t hd = (size_t)kv->heads * kHeadDim;
-    // Single tokens run on the split-KV decode, a row per unit; other calls on a bf16 cache in blocks
-    // of rows, split over the keys.
-    const bool tokens = !tree && n_rows == n_seq, few = !tokens && cache_bf16, out_bf16 = out_dtype == PTTS_B200_BF16;
+    // Single tokens run on the split-KV decode, a row per unit; up to 64 rows a sequence on a bf16
+    // cache in blocks of rows, split over the keys; longer prompts in tiles of 128 rows.
+    const int most = *std::max_element(rows_host, rows_host + n_seq);
+    const bool tokens = !tree && n_rows == n_seq, few = !tokens && cache_bf16 && most <= kTreeNodes;
+    const bool prompt = !tokens && cache_bf16 && !few, out_bf16 = out_dtype == PTTS_B200_BF16;
     int block = 0, grid = sm_count(kv->device);
     std::vector<int2> blocks;
+    if (prompt) blocks = make_tiles(offsets, streams_host, kv->h_len);
     if (few) {
-        block = score_rows_block(*std::max_element(rows_host, rows_host + n_seq));
+        block = score_rows_block(most);
         grid = score_rows_grid(block, kv->heads, grid);
         for (int i = 0; i < n_seq; ++i)
             for (int r = offsets[i]; r < offsets[i + 1]; r += block)
@@ -676,7 +679,7 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
         p.unit_lo = p.prefix + p.n_units + 1;
         p.cta_first = p.unit_lo + p.n_units;
     }
-    if (few) {  // two bf16 planes in the f32 buffer
+    if (few || prompt) {  // two bf16 planes in the f32 buffer
         p.q_hi = reinterpret_cast<__nv_bfloat16*>(p.q_out);
         p.q_lo = p.q_hi + (size_t)n_rows * hd;
         p.q_scale = score_q_scale(sc.softcap, !out_bf16);
@@ -739,6 +742,30 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
         a.err = p.err;
         require(launch_score_rows(a, block, grid, s), PTTS_B200_ERR_CUDA,
                 "could not describe the cache's tensors (cuTensorMapEncodeTiled)");
+        check_launch();
+        return;
+    }
+    if (prompt) {
+        ScorePromptArgs a{};
+        a.k_cache = p.k_cache;
+        a.v_cache = p.v_cache;
+        a.q_hi = p.q_hi;
+        a.q_lo = p.q_lo;
+        a.out = out;
+        a.out_bf16 = out_bf16;
+        a.ld = (int)hd;
+        a.heads = kv->heads;
+        a.num_streams = kv->streams;
+        a.capacity = kv->capacity;
+        a.n_rows = n_rows;
+        a.rows = p.rows;
+        a.rule.cap = sc.softcap;
+        a.rule.slopes = sc.slopes;
+        a.tiles = reinterpret_cast<const int2*>(d + blocks_at);
+        a.n_tiles = (int)blocks.size();
+        a.err = p.err;
+        require(launch_score_prompt(a, s), PTTS_B200_ERR_CUDA,
+                "could not describe the prompt attention's tensors (cuTensorMapEncodeTiled)");
         check_launch();
         return;
     }

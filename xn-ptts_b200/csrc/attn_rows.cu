@@ -73,8 +73,7 @@ __device__ __forceinline__ void ldsm_x4_t(uint32_t a, uint32_t* r) {
                  : "r"(a));
 }
 __device__ __forceinline__ void mma_bf16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -85,14 +84,6 @@ __device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int y,
         "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(y), "r"(z), "r"(smem_u32(bar)), "l"(policy)
         : "memory");
 }
-// Takes the bf16s that are not finite out of a pair; whether there was one.
-__device__ __forceinline__ bool drop_not_finite(uint32_t& u) {
-    const bool lo = (u & 0x7f80u) == 0x7f80u, hi = (u & 0x7f800000u) == 0x7f800000u;
-    u = lo ? u & 0xffff0000u : u;
-    u = hi ? u & 0x0000ffffu : u;
-    return lo || hi;
-}
-
 // The slots a row sees, for chunks that some row does not see whole.
 struct Sees {
     int lo, hi, base;
@@ -191,7 +182,8 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
     const bool biased = a.rule.slopes != nullptr;
     uint32_t qh[MT][4][4], ql[MT][4][4];
     float o[MT][8][4], m[MT][2], l[MT][2], posf[MT][2];
-    int full_lo = 0, full_hi = -1, tiles = 0;
+    int full_lo = 0, full_hi = -1;
+    bool any = false;  // this warp has rows of the block
     // ldmatrix addresses within a head's tile: K takes 8 keys x 32 dims a time (matrix = dims), V
     // 16 keys x 16 dims (matrices: keys, then dims).
     const int k_row = lane & 7, k_chunk = lane >> 3;
@@ -204,9 +196,8 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
         }
         const RowsHdr hd = *reinterpret_cast<const RowsHdr*>(hdrs + st * 64);
         if (hd.flags & kREnd) break;
-        const int mine = hd.nrows - rbase;  // this warp's rows, if positive
         if (hd.flags & kRFirst) {
-            tiles = mine <= 0 ? 0 : min(MT, (mine + 15) / 16);
+            any = rbase < hd.nrows;
             full_lo = 0, full_hi = 0x7fffffff;
 #pragma unroll
             for (int i = 0; i < MT; ++i)
@@ -245,7 +236,7 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
         const unsigned char* kt = smem + st * S::kStageBytes + hl * kHeadTile;
         const uint32_t ka = smem_u32(kt), va = ka + S::kStageBytes / 2;
         const bool edge = hd.n < KC || hd.slot < full_lo || hd.slot + KC - 1 > full_hi;
-        if (tiles > 0) {
+        if (any) {
             // S = Q K^T: key 8 n + 2 t (+1) of rows g and g + 8 in s[i][n][0..3].
             float s[MT][4][4];
 #pragma unroll
@@ -254,26 +245,31 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
                 for (int n = 0; n < 4; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[i][n][e] = 0.f;
+            // A dims half at a time, its eight accumulators in turn: each mma waits for the one before
+            // it on the same accumulator, 8 (or 4) back.
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
+            for (int hf = 0; hf < 2; ++hf) {
+                uint32_t kb[4][4];
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    uint32_t kb[4];
+                for (int n = 0; n < 4; ++n) {
                     const int key = 8 * n + k_row;
-                    ldsm_x4(ka + key * 128 + (((4 * hf + k_chunk) ^ (key & 7)) << 4), kb);
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        if (i > 0 && i >= tiles) continue;
-                        mma_bf16(s[i][n], qh[i][2 * hf], kb[0], kb[1]);
-                        mma_bf16(s[i][n], ql[i][2 * hf], kb[0], kb[1]);
-                        mma_bf16(s[i][n], qh[i][2 * hf + 1], kb[2], kb[3]);
-                        mma_bf16(s[i][n], ql[i][2 * hf + 1], kb[2], kb[3]);
-                    }
+                    ldsm_x4(ka + key * 128 + (((4 * hf + k_chunk) ^ (key & 7)) << 4), kb[n]);
                 }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) mma_bf16(s[i][n], qh[i][2 * hf + k], kb[n][2 * k], kb[n][2 * k + 1]);
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) mma_bf16(s[i][n], ql[i][2 * hf + k], kb[n][2 * k], kb[n][2 * k + 1]);
+                }
+            }
             // Rules.
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                if (i > 0 && i >= tiles) continue;
 #pragma unroll
                 for (int n = 0; n < 4; ++n)
 #pragma unroll
@@ -325,7 +321,7 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
 #pragma unroll
                     for (int n = 1; n < 4; ++n) x = fmaxf(x, fmaxf(s[i][n][2 * b], s[i][n][2 * b + 1]));
                     mt[i][b] = x;
-                    raise |= i < tiles && x > m[i][b] + kRaise;
+                    raise |= x > m[i][b] + kRaise;
                 }
             if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -375,7 +371,6 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
                     }
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
-                        if (i > 0 && i >= tiles) continue;
                         mma_bf16(o[i][2 * d2], ph[i][kk], vb[0], vb[1]);
                         mma_bf16(o[i][2 * d2 + 1], ph[i][kk], vb[2], vb[3]);
                         if constexpr (P2) {
@@ -405,7 +400,7 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[st]);
-        if (!(hd.flags & kRLast) || tiles == 0) continue;
+        if (!(hd.flags & kRLast) || !any) continue;
         // The end of this CTA's piece of the block.
 #pragma unroll
         for (int i = 0; i < MT; ++i)
@@ -449,44 +444,44 @@ __global__ void __launch_bounds__(256) score_rows_merge_kernel(ScoreRowsArgs a, 
     const int c0 = cta_of(pb, total, G), c1 = cta_of(pe - 1, total, G);
     if (c0 == c1) return;
     const int2 rows = a.blocks[u];
-    for (int r = threadIdx.x >> 5; r < rows.y; r += 8) {
-        auto rec = [&](int c) {
-            return a.part + (((long long)(2 * c + (c == c0 ? 1 : 0)) * a.heads + head) * rows_max + r) * kPartStride;
-        };
-        float mx = kScoreLow;
-        for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, rec(c)[64]);
+    const int r = blockIdx.z * 8 + (threadIdx.x >> 5);
+    if (r >= rows.y) return;
+    auto rec = [&](int c) {
+        return a.part + (((long long)(2 * c + (c == c0 ? 1 : 0)) * a.heads + head) * rows_max + r) * kPartStride;
+    };
+    float mx = kScoreLow;
+    for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, rec(c)[64]);
 #pragma unroll
-        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        float den = 0.f, x0 = 0.f, x1 = 0.f;
-        for (int cb = c0; cb <= c1; cb += 32) {
-            const int n = min(32, c1 - cb + 1);
-            float w = 0.f;
-            if (lane < n) {
-                const float2 ml = *reinterpret_cast<const float2*>(rec(cb + lane) + 64);
-                w = score_exp2(ml.x - mx);
-                den += w * ml.y;
-            }
-#pragma unroll 8
-            for (int i = 0; i < n; ++i) {
-                const float f = __shfl_sync(0xffffffffu, w, i);
-                const float2 v = *reinterpret_cast<const float2*>(rec(cb + i) + 2 * lane);
-                x0 = fmaf(f, v.x, x0);
-                x1 = fmaf(f, v.y, x1);
-            }
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    float den = 0.f, x0 = 0.f, x1 = 0.f;
+    for (int cb = c0; cb <= c1; cb += 32) {
+        const int n = min(32, c1 - cb + 1);
+        float w = 0.f;
+        if (lane < n) {
+            const float2 ml = *reinterpret_cast<const float2*>(rec(cb + lane) + 64);
+            w = score_exp2(ml.x - mx);
+            den += w * ml.y;
         }
-        den = warp_sum(den);
-        const float inv = den == 0.f ? 0.f : 1.f / den;
-        const long long at = (long long)(rows.x + r) * a.ld + head * kHeadDim + 2 * lane;
-        if constexpr (P2) *reinterpret_cast<float2*>(static_cast<float*>(a.out) + at) = make_float2(x0 * inv, x1 * inv);
-        else *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + at) = pack_bf16x2(x0 * inv, x1 * inv);
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+            const float f = __shfl_sync(0xffffffffu, w, i);
+            const float2 v = *reinterpret_cast<const float2*>(rec(cb + i) + 2 * lane);
+            x0 = fmaf(f, v.x, x0);
+            x1 = fmaf(f, v.y, x1);
+        }
     }
+    den = warp_sum(den);
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    const long long at = (long long)(rows.x + r) * a.ld + head * kHeadDim + 2 * lane;
+    if constexpr (P2) *reinterpret_cast<float2*>(static_cast<float*>(a.out) + at) = make_float2(x0 * inv, x1 * inv);
+    else *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + at) = pack_bf16x2(x0 * inv, x1 * inv);
 }
 
 template <class S, int CAP, bool P2>
 void launch_shape(const ScoreRowsArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int grid, cudaStream_t s) {
     set_max_dynamic_smem(reinterpret_cast<const void*>(score_rows_kernel<S, CAP, P2>), S::kSmem);
     launch_k(score_rows_kernel<S, CAP, P2>, dim3(grid, a.heads / S::kHeads), dim3(kThreadsR), S::kSmem, s, a, mk, mv);
-    if (grid > 1) launch_k(score_rows_merge_kernel<P2>, dim3(a.n_units, a.heads), dim3(256), 0, s, a, grid, S::kRows);
+    if (grid > 1) launch_k(score_rows_merge_kernel<P2>, dim3(a.n_units, a.heads, S::kRows / 8), dim3(256), 0, s, a, grid, S::kRows);
 }
 
 template <class S>

@@ -36,4 +36,12 @@ __device__ __forceinline__ float cap_fast(float x, float cap) {
     return fmaf(-2.f * c, r, c);
 }
 
+// Takes the bf16s that are not finite out of a pair; whether there was one.
+__device__ __forceinline__ bool drop_not_finite(uint32_t& u) {
+    const bool lo = (u & 0x7f80u) == 0x7f80u, hi = (u & 0x7f800000u) == 0x7f800000u;
+    u = lo ? u & 0xffff0000u : u;
+    u = hi ? u & 0x0000ffffu : u;
+    return lo || hi;
+}
+
 }  // namespace ptts

@@ -121,6 +121,24 @@ int score_rows_grid(int block, int heads, int sms);  // CTAs along the keys (the
 size_t score_rows_part_floats(int block, int heads, int grid);
 bool launch_score_rows(const ScoreRowsArgs& a, int block, int grid, cudaStream_t s);
 
+// Prompts on tcgen05, bf16 caches (attn_score_prompt.cu): tiles (first row, rows) of up to 128 rows
+// of one sequence. False: the tensor maps could not be made, nothing launched.
+struct ScorePromptArgs {
+    const void* k_cache;  // the layer
+    const void* v_cache;
+    const __nv_bfloat16* q_hi;  // [n_rows][ld], scaled by score_q_scale
+    const __nv_bfloat16* q_lo;
+    void* out;            // [n_rows][ld]
+    bool out_bf16;
+    int ld, heads, num_streams, capacity, n_rows;
+    ScoreRows rows;       // no lineages
+    ScoreRule rule;
+    const int2* tiles;
+    int n_tiles;
+    uint32_t* err;
+};
+bool launch_score_prompt(const ScorePromptArgs& a, cudaStream_t s);
+
 // Acceptance: per stream the accepted nodes' rows move from slot len + node[j] to len + j, in
 // every layer and head group, and the length becomes len + their number. Nodes rise, so
 // node[j] >= j. The lists are one array of int32 (host or device): streams [n], lengths before
