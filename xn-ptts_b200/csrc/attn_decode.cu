@@ -342,6 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_attn_kernel(DecodeArgs a) 
     // Below every score of the plain op's inputs; a bias can carry scores further down.
     constexpr float kLow = SCORED ? kScoreLow : -1e30f;
     float q[8], m = kLow, l = 0.f, acc[8];
+    const float inv_cap = SCORED && a.cap > 0.f ? 1.f / a.cap : 0.f;
     const float slope = SCORED && a.slopes ? a.slopes[h] : 0.f;
     // The q of the CTA's first piece (stream cta_first[c]), loaded now rather than staged.
     float q_first[8];
@@ -421,8 +422,8 @@ __global__ void __launch_bounds__(kThreads, 1) decode_attn_kernel(DecodeArgs a) 
                 d1 += __shfl_xor_sync(0xffffffffu, d1, o);
             }
             if constexpr (SCORED) {
-                d0 = score_exact(d0, a.cap, slope, hd.at - p - r0);
-                d1 = score_exact(d1, a.cap, slope, hd.at - p - r1);
+                d0 = score_exact(d0, a.cap, inv_cap, slope, hd.at - p - r0);
+                d1 = score_exact(d1, a.cap, inv_cap, slope, hd.at - p - r1);
             }
             if (r0 >= n) d0 = -INFINITY;
             if (r1 >= n) d1 = -INFINITY;

@@ -270,15 +270,13 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
             // Rules.
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
+                if (CAP == kCapFast) cap_fast<16>(&s[i][0][0], a.rule.cap);
+                if (CAP == kCapExact) {
 #pragma unroll
-                for (int n = 0; n < 4; ++n)
+                    for (int n = 0; n < 4; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float x = s[i][n][e];
-                        if (CAP == kCapFast) x = cap_fast(x, a.rule.cap);
-                        if (CAP == kCapExact) x = cap_exact(x, a.rule.cap);
-                        s[i][n][e] = x;
-                    }
+                        for (int e = 0; e < 4; ++e) s[i][n][e] = cap_exact(s[i][n][e], a.rule.cap);
+                }
                 if (biased && !edge) {
 #pragma unroll
                     for (int n = 0; n < 4; ++n)

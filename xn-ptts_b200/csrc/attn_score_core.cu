@@ -21,6 +21,7 @@ __global__ void __launch_bounds__(256) score_core_kernel(ScoreCoreArgs a) {
     const unsigned long long lineage = a.rows.lineage ? a.rows.lineage[row] : 0;
     const int base = a.rows.lineage ? a.rows.base[row] : 0x7fffffff;
     const float slope = a.rule.slopes ? a.rule.slopes[h] : 0.f;
+    const float inv_cap = a.rule.cap > 0.f ? 1.f / a.rule.cap : 0.f;
     float q[8], m = kScoreLow, l = 0.f, acc[8];
     const long long at = ((long long)row * a.heads + h) * kHeadDim + 8 * j;
 #pragma unroll
@@ -42,9 +43,9 @@ __global__ void __launch_bounds__(256) score_core_kernel(ScoreCoreArgs a) {
         }
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+        const int kp = seen && node ? a.rows.pos[a.rows.row0[row] + slot - base] : slot;
+        d = score_exact(d, a.rule.cap, inv_cap, slope, pos - kp);
         if (seen) {
-            const int kp = node ? a.rows.pos[a.rows.row0[row] + slot - base] : slot;
-            d = score_exact(d, a.rule.cap, slope, pos - kp);
             const float mn = fmaxf(m, d);
             const float corr = score_exp2(m - mn), e = score_exp2(d - mn);
             l = fmaf(l, corr, e);

@@ -1,28 +1,31 @@
 // Attention with score rules for prompts, bf16 caches, on tcgen05: one CTA per (tile of up to 128
-// query rows of one sequence, head), two CTAs on an SM.
+// query rows of one sequence, 1 to 8 heads one after another), two CTAs on an SM.
 //
-// Bound by the softmax's exponentials: a 128 x 128 tile has 16,384 scores for 2 x 2.1 MFLOP, and an
-// SM makes 16 exp2 a cycle (1024 cycles a tile) while the tensor cores need 512 cycles for S (q as
-// a bf16 hi/lo pair) and 256 for P V. So the products hide behind the softmax of the other CTA on
-// the SM, whose items run half a step apart, and one CTA keeps a plain order per 128-key item:
-//   warps 0-3  a thread per query row (TMEM lane): S from TMEM, rules and mask, the row's maximum
-//              (raised only when a score passes it by 2^8, the one time O is rescaled, in TMEM), P as
-//              bf16 into TMEM, the row's sum in f32; at the end O / l to the output.
-//   warp 4     one lane issues S = Q K^T (both planes of q) and O += P V with P from TMEM. The next
-//              item's S goes ahead of this item's P V: the softmax waits for S alone.
-//   warp 5     one lane copies the Q tile once and each item's K and V by TMA into two-slot rings.
-// A row per thread leaves nothing to exchange between threads. The scores are read twice from TMEM
-// (for the maximum, then for P): keeping 128 of them in registers would leave no room for two CTAs.
-// Where a cap up to kBoundedCap bounds the scores there is no maximum pass: exp2 runs against the
-// row's nearest key's bias, which the largest score passes by at most cap x log2(e) < 58 either way.
+// Bound by the softmax: a 128 x 128 tile has 16,384 scores for 2 x 2.1 MFLOP. An SM makes 16 exp2 a
+// cycle (1024 cycles a tile) and issues 4 to 9 instructions a score on 128 lanes (500 to 1200),
+// while the tensor cores need 512 cycles for S (q as a bf16 hi/lo pair) and 256 for P V.
+//   warps 0-7  two threads per query row (TMEM lane), 64 of the item's 128 keys and 32 dims each: the
+//              scores from TMEM into registers, rules and mask, the row's maximum (the halves agree by
+//              one barrier that it stays; it is raised, and O rescaled in TMEM, only when a score passes
+//              it by 2^8), P as bf16 into TMEM, the row's sum in f32; at a head's end O / l to the output.
+//   warp 8     one lane issues S = Q K^T (both planes of q) and O += P V with P from TMEM. The next
+//              item's S starts as soon as the softmax holds this one's in registers.
+//   warp 9     one lane copies each head's Q tile and each item's K and V (128 keys) by TMA, K and V
+//              in two-slot rings, so the next head's data come during this head's last item.
+// Two threads a row and two CTAs an SM make four softmax warps a scheduler, which fill each other's
+// waits (with a thread a row, half as many, the issue slots were 35 to 46 % used). Where a cap up to
+// kBoundedCap bounds the scores there is no maximum: exp2 runs against the bias of the row's nearest
+// key, which a score passes by at most cap x log2(e) < 58 either way. Items run from the last keys to
+// the first: a causal row's nearest keys, whose bias is the least, set the maximum at once.
 //
 // f32 outputs hold P as a bf16 hi/lo pair over the columns of S (its next item waits for P V);
 // bf16 outputs round P once to bf16, as the output itself is rounded.
 //
 // Items start at the first slot any row of the tile sees and end at the last. An item that some row
-// does not see whole masks scores by a 32-bit word per 32 keys (32 keys that no row of a warp sees
-// are skipped), and takes values that are not finite, or that no row sees, out of the V tile: 0 x
-// NaN is NaN. Rows that do see such a value get it back at the end, from the cache.
+// does not see whole masks scores by a 32-bit word per 32 keys (32 keys that no row of a warp sees are
+// passed over), and takes values that are not finite,
+// or that no row sees, out of the V tile: 0 x NaN is NaN. Rows that do see such a value get it back at
+// the end, from the cache.
 #include "common.cuh"
 #include "fa_tc.cuh"
 #include "score.cuh"
@@ -32,7 +35,10 @@ namespace ptts {
 namespace {
 
 constexpr int QT = 128, KT = 128;
-constexpr int kMmaW = 4, kLoadW = 5, kThreadsP = 192;
+constexpr int kSoftW = 4, kMmaW = kSoftW, kLoadW = kSoftW + 1;
+// Two warpgroups: the softmax takes most of the launch's 256 x 128 registers (128 scores a thread).
+constexpr int kThreadsP = 256, kRegsP = 128, kRegsSoft = 200, kRegsRest = 56;
+static_assert(128 * (kRegsSoft + kRegsRest) <= kThreadsP * kRegsP, "the split fits the launch");
 constexpr int kTile = 128 * 128;  // bytes of a Q plane, a K tile or a V tile: 128 rows x 64 bf16
 constexpr int kSlots = 2;
 constexpr int kOffK = 2 * kTile, kOffV = kOffK + kSlots * kTile, kOffBars = kOffV + kSlots * kTile;
@@ -44,10 +50,11 @@ constexpr uint32_t kIdescPV = (1u << 4) | (1u << 7) | (1u << 10) | (8u << 17) | 
 constexpr float kRaiseP = 8.f;
 constexpr float kBoundedCap = 40.f;  // 40 log2(e) < 58: weights and sums of 2^58 stay far inside f32 and bf16
 
-// Single buffers for S, P and O: item i completes phase i of sfull, pfull and odone, and each waiter
-// asks for every phase (or one that the last wait on another implies), so none is two behind.
+// Single buffers for S, P and O: item i completes phase i of sfull, sfree, pfull and odone, head hh
+// phase hh of qready and qfree, and each waiter asks for every phase (or for one that its last wait on
+// another implies), so none is two behind.
 struct Bars {
-    uint64_t qready, kfull[kSlots], kempty[kSlots], vfull[kSlots], vempty[kSlots], sfull, pfull, odone;
+    uint64_t qready, kfull[kSlots], kempty[kSlots], vfull[kSlots], vempty[kSlots], qfree, sfull, sfree, pfull, odone;
 };
 
 __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t* r) {
@@ -57,29 +64,19 @@ __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t* r) {
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
-__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// 32 scores of a row (keys slot .. slot + 31) with the rules: capped, biased, and -inf where `seen`
-// has no bit.
-template <int CAP, bool BIAS>
-__device__ __forceinline__ void apply_rules(float* s, float cap, float slope, float ahead, uint32_t seen) {
-    if (CAP == kCapFast) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) s[j] = cap_fast(s[j], cap);
-    }
-    if (CAP == kCapExact) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) s[j] = cap_exact(s[j], cap);
-    }
-    if (BIAS) {  // ahead = position - slot
-#pragma unroll
-        for (int j = 0; j < 32; ++j) s[j] = fmaf(-slope, fabsf(ahead - (float)j), s[j]);
-    }
-    if (seen != 0xffffffffu) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) s[j] = seen >> j & 1 ? s[j] : -INFINITY;
-    }
+__device__ __forceinline__ void ld16(uint32_t taddr, float* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+        : "r"(taddr));
 }
+__device__ __forceinline__ void ld8(uint32_t taddr, float* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // The values of slots lo .. hi that are not finite, from the cache, onto 32 dims of a row.
 __device__ __forceinline__ void add_not_finite(const ScorePromptArgs& a, int kv_row, int x, int lo, int hi, float* o) {
@@ -90,6 +87,97 @@ __device__ __forceinline__ void add_not_finite(const ScorePromptArgs& a, int kv_
             const float y = __bfloat162float(v[j]);
             if (!isfinite(y)) o[j] += y;
         }
+}
+
+// Key `key` of a V tile: zeros if the key is gone, else without what is not finite
+// (x 0 is NaN then), which `bad` records. Swizzled 16-byte chunks; visible to the products afterwards.
+__device__ __forceinline__ void clean_v(unsigned char* tile, int key, bool gone, int* bad) {
+    uint4* v = reinterpret_cast<uint4*>(tile + key * 128);
+    const uint32_t zero = 0;
+    uint32_t probe = 0;
+    uint4 w[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+        w[c] = v[c ^ (key & 7)];
+        const uint32_t* u = &w[c].x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(probe) : "r"(u[j]), "r"(zero));
+    }
+    const bool drop = (probe & 0x7fff7fffu) != 0;  // NaN in either half
+    if (gone || drop) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            uint32_t* u = &w[c].x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (gone) u[j] = 0u;
+                else drop_not_finite(u[j]);
+            }
+            v[c ^ (key & 7)] = w[c];
+        }
+        if (!gone) *bad = 1;
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+// 32 scores of a row: capped, biased (`ahead` = position - first key), -inf outside keys from .. to
+// (unless `whole`: every key is visible).
+template <int CAP, bool BIAS>
+__device__ __forceinline__ void rules(float* s, float cap, float slope, int ahead, int from, int to, bool whole) {
+    if (CAP == kCapFast) cap_fast<32>(s, cap);
+    if (CAP == kCapExact) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) s[j] = cap_exact(s[j], cap);
+    }
+    if (BIAS && __all_sync(0xffffffffu, ahead >= 31)) {  // no key ahead of its row: slope j - slope ahead
+        const float at = -slope * (float)ahead;
+        const float2 at2 = make_float2(at, at);
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+            const float2 t = __fadd2_rn(make_float2(s[j], s[j + 1]), at2);
+            s[j] = fmaf(slope, (float)j, t.x);
+            s[j + 1] = fmaf(slope, (float)(j + 1), t.y);
+        }
+    } else if (BIAS) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) s[j] = fmaf(-slope, fabsf((float)ahead - (float)j), s[j]);
+    }
+    if (!whole && __any_sync(0xffffffffu, from > 0 || to < 31)) {
+        const uint32_t x = from <= 0 ? 0xffffffffu : (from > 31 ? 0u : 0xffffffffu << from);
+        const uint32_t y = to >= 31 ? 0xffffffffu : (to < 0 ? 0u : 0xffffffffu >> (31 - to));
+#pragma unroll
+        for (int j = 0; j < 32; ++j) s[j] = (x & y) >> j & 1 ? s[j] : -INFINITY;
+    }
+}
+// The item's scores are in this warp's registers: S may take the next item's.
+__device__ __forceinline__ void s_is_read(Bars* b, int lane) {
+    fa_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&b->sfree);
+}
+__device__ __forceinline__ float most_of(const float* s) {  // four chains of three-input maxima
+    float m[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const float* x = s + 8 * q;
+        m[q] = fmaxf(fa_max3(fa_max3(fa_max3(x[0], x[1], x[2]), x[3], x[4]), x[5], x[6]), x[7]);
+    }
+    return fmaxf(fa_max3(m[0], m[1], m[2]), m[3]);
+}
+// Half c (32 dims) of a head's output row.
+template <bool P2>
+__device__ __forceinline__ void store_half(const ScorePromptArgs& a, int row, int head, int c, const float* o) {
+    const long long at = (long long)row * a.ld + head * kHeadDim + 32 * c;
+    if constexpr (P2) {
+        float4* out = reinterpret_cast<float4*>(static_cast<float*>(a.out) + at);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) out[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+    } else {
+        uint4* out = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + at);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            out[j] = make_uint4(pack_bf16x2(o[8 * j], o[8 * j + 1]), pack_bf16x2(o[8 * j + 2], o[8 * j + 3]),
+                                pack_bf16x2(o[8 * j + 4], o[8 * j + 5]), pack_bf16x2(o[8 * j + 6], o[8 * j + 7]));
+    }
 }
 
 // BOUNDED: the cap bounds the scores, no maximum is taken.
@@ -103,7 +191,7 @@ __global__ void __launch_bounds__(kThreadsP, 2) score_prompt_kernel(ScorePromptA
     unsigned char* sm = smem_raw + (base - raw);
     Bars* b = reinterpret_cast<Bars*>(sm + kOffBars);
     __shared__ uint32_t s_tmem;
-    __shared__ int s_lo[4], s_hi[4], s_lo_most[4], s_hi_least[4], s_bad, s_k_issued, s_v_issued;
+    __shared__ int s_lo[4], s_hi[4], s_lo_most[4], s_hi_least[4], s_bad, s_q_issued, s_k_issued, s_v_issued;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         mbar_init(&b->qready, 1);
@@ -113,10 +201,12 @@ __global__ void __launch_bounds__(kThreadsP, 2) score_prompt_kernel(ScorePromptA
             mbar_init(&b->vfull[i], 1);
             mbar_init(&b->vempty[i], 1);
         }
+        mbar_init(&b->qfree, 1);
         mbar_init(&b->sfull, 1);
-        mbar_init(&b->pfull, 4);
+        mbar_init(&b->sfree, kSoftW);
+        mbar_init(&b->pfull, kSoftW);
         mbar_init(&b->odone, 1);
-        s_bad = s_k_issued = s_v_issued = 0;
+        s_bad = s_q_issued = s_k_issued = s_v_issued = 0;
         fence_mbar_init();
     }
     if (warp == 0) {
@@ -126,15 +216,16 @@ __global__ void __launch_bounds__(kThreadsP, 2) score_prompt_kernel(ScorePromptA
     }
     grid_dep_wait();
     grid_dep_launch();
-    const int head = blockIdx.x % a.heads;
-    const int2 tile = a.tiles[blockIdx.x / a.heads];
+    const int slabs = a.heads / a.heads_per_cta, head0 = blockIdx.x % slabs * a.heads_per_cta;
+    const int2 tile = a.tiles[blockIdx.x / slabs];
     const int row0 = tile.x, nrows = tile.y;
     // The row of each softmax thread, and the slots the tile's rows see: any (min lo .. max hi) and
     // all (max lo .. min hi).
     int lo = 0, hi = -1;
-    const bool there = tid < nrows;
-    if (warp < 4) {
-        if (there) lo = a.rows.lo[row0 + tid], hi = a.rows.hi[row0 + tid];
+    const int r = tid;  // softmax threads: row r
+    const bool there = r < nrows;
+    if (warp < kSoftW) {
+        if (there) lo = a.rows.lo[row0 + r], hi = a.rows.hi[row0 + r];
         const bool sees = lo <= hi;
         const int x0 = __reduce_min_sync(0xffffffffu, sees ? lo : 0x7fffffff), x1 = __reduce_max_sync(0xffffffffu, sees ? hi : -1);
         const int y0 = __reduce_max_sync(0xffffffffu, there ? lo : 0), y1 = __reduce_min_sync(0xffffffffu, there ? hi : 0x7fffffff);
@@ -149,110 +240,111 @@ __global__ void __launch_bounds__(kThreadsP, 2) score_prompt_kernel(ScorePromptA
     const int lo_most = max(max(s_lo_most[0], s_lo_most[1]), max(s_lo_most[2], s_lo_most[3]));
     const int hi_least = min(min(s_hi_least[0], s_hi_least[1]), min(s_hi_least[2], s_hi_least[3]));
     const int sid = a.rows.stream[row0];
-    const int n = sid < 0 || end <= 0 ? 0 : (end - first + KT - 1) / KT;
-    // The head's rows of this stream in the layer: [group][stream][slot] rows of 8 heads.
-    const int kv_row = (int)(((long long)(head / kGroupHeads) * a.num_streams + max(sid, 0)) * a.capacity);
-    const int kv_x = (head % kGroupHeads) * kHeadDim;
+    // Items: n key tiles for each of the CTA's heads; item i is key tile i % n of head head0 + i / n.
+    const int n = sid < 0 || end <= 0 ? 0 : (end - first + KT - 1) / KT, items = n * a.heads_per_cta;
+    // A head's rows of this stream in the layer: [group][stream][slot] rows of 8 heads.
+    auto kv_row = [&](int head) {
+        return (int)(((long long)(head / kGroupHeads) * a.num_streams + max(sid, 0)) * a.capacity);
+    };
+    auto kv_x = [&](int head) { return (head % kGroupHeads) * kHeadDim; };
 
-    if (warp < 4) {
+    if (warp < kSoftW) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoft));
         const uint32_t lanes = tmem + ((uint32_t)(32 * warp) << 16);
-        const float slope = BIAS ? a.rule.slopes[head] * kScoreLog2e : 0.f;
-        const int pos = BIAS && there ? a.rows.pos[row0 + tid] : 0;
-        // BOUNDED: exp2 against the bias of the nearest visible key.
-        float m = BOUNDED ? (BIAS ? -slope * (float)max(max(lo - pos, pos - hi), 0) : 0.f) : kScoreLow, l = 0.f;
+        const int pos = BIAS && there ? a.rows.pos[row0 + r] : 0;
+        const float2 minus1 = make_float2(-1.f, -1.f);
+        float m = 0.f, l = 0.f, slope = 0.f;
         bool ok = true;
-        for (int i = 0; i < n; ++i) {
-            const int k0 = first + i * KT;
+        if (n == 0 && there) {  // no row sees anything: zeros
+            float o[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = 0.f;
+            for (int hh = 0; hh < a.heads_per_cta; ++hh) {
+                store_half<P2>(a, row0 + r, head0 + hh, 0, o);
+                store_half<P2>(a, row0 + r, head0 + hh, 1, o);
+            }
+        }
+        for (int i = 0, kt = 0, head = head0; i < items; ++i) {
+            if (kt == 0) {
+                if (BIAS) slope = a.rule.slopes[head] * kScoreLog2e;
+                // BOUNDED: exp2 against the bias of the nearest visible key.
+                m = BOUNDED ? (BIAS ? -slope * (float)max(max(lo - pos, pos - hi), 0) : 0.f) : kScoreLow;
+                l = 0.f;
+            }
+            const int k0 = first + (n - 1 - kt) * KT;
             ok = __all_sync(0xffffffffu, mbar_wait(&b->sfull, i & 1));
             if (!ok) break;
             fa_after();
-            // This row's visible keys of the item, a bit each.
-            uint32_t seen[4];
+            // Whether some row of the warp sees some of each 32 keys; every row every key: `whole`.
+            const bool whole = k0 >= lo_most && k0 + KT - 1 <= hi_least;
+            uint32_t alive = 0xfu;
+            if (!whole) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int x = lo - k0 - 32 * c, y = hi - k0 - 32 * c;  // bits x .. y
-                const uint32_t from = x <= 0 ? 0xffffffffu : (x > 31 ? 0u : 0xffffffffu << x);
-                const uint32_t to = y >= 31 ? 0xffffffffu : (y < 0 ? 0u : 0xffffffffu >> (31 - y));
-                seen[c] = from & to;
+                for (int c = 0; c < 4; ++c)
+                    if (!__any_sync(0xffffffffu, lo <= k0 + 32 * c + 31 && hi >= k0 + 32 * c)) alive &= ~(1u << c);
             }
+            float s[BOUNDED ? 32 : KT];
+            bool waited = i == 0;  // for P V of the item before
             if (!BOUNDED) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) fa_ld32(lanes + kColS + 32 * c, s + 32 * c);
+                fa_wait_ld();
+                if (!P2) s_is_read(b, lane);
                 float mt = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if (!__any_sync(0xffffffffu, seen[c] != 0)) continue;
-                    float s[32];
-                    fa_ld32(lanes + kColS + 32 * c, s);
-                    fa_wait_ld();
-                    const bool whole = __all_sync(0xffffffffu, seen[c] == 0xffffffffu);
-                    apply_rules<CAP, BIAS>(s, a.rule.cap, slope, (float)(pos - k0 - 32 * c), whole ? 0xffffffffu : seen[c]);
-                    float m4[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const float* sq = s + 8 * q;
-                        m4[q] = fa_max3(fa_max3(fa_max3(sq[0], sq[1], sq[2]), sq[3], sq[4]), sq[5], sq[6]);
-                        m4[q] = fmaxf(m4[q], sq[7]);
+                for (int c = 0; c < 4; ++c)
+                    if (alive >> c & 1) {
+                        rules<CAP, BIAS>(s + 32 * c, a.rule.cap, slope, pos - k0 - 32 * c, lo - k0 - 32 * c, hi - k0 - 32 * c, whole);
+                        mt = fmaxf(mt, most_of(s + 32 * c));
                     }
-                    mt = fmaxf(mt, fmaxf(fa_max3(m4[0], m4[1], m4[2]), m4[3]));
-                    if (CAP != kCapNone || BIAS) {  // the second pass takes the scores as they are now
-                        uint32_t w[32];
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(s[j]);
-                        fa_st32(lanes + kColS + 32 * c, w);
-                    }
-                }
-                if (CAP != kCapNone || BIAS) wait_st();
                 const bool raise = mt > m + kRaiseP;
                 if (__any_sync(0xffffffffu, raise)) {
                     const float mn = raise ? mt : m, f = score_exp2(m - mn);
                     l *= f;
                     m = mn;
-                    if (i > 0) {  // O holds the items before this one once their P V is done
+                    if (kt > 0) {  // O holds the head's items before this one once their P V is done
                         ok = __all_sync(0xffffffffu, mbar_wait(&b->odone, (i - 1) & 1));
                         if (!ok) break;
+                        waited = true;
                         fa_after();
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            float o[32];
-                            uint32_t w[32];
-                            fa_ld32(lanes + kColO + 32 * c, o);
+#pragma unroll 1
+                        for (int c = 0; c < 8; ++c) {
+                            float o[8];
+                            uint32_t w[8];
+                            ld8(lanes + kColO + 8 * c, o);
                             fa_wait_ld();
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(o[j] * f);
-                            fa_st32(lanes + kColO + 32 * c, w);
+                            for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(o[j] * f);
+                            fa_st8(lanes + kColO + 8 * c, w);
                         }
                         wait_st();
                     }
                 }
             }
-            if (!P2 && i > 0) {  // P V of the item before has read P (a raise has waited for it already)
+            if (!P2 && !waited) {  // P V of the item before has read P
                 ok = __all_sync(0xffffffffu, mbar_wait(&b->odone, (i - 1) & 1));
                 if (!ok) break;
                 fa_after();
             }
             // P, 32 keys at a time: bf16 pairs into its own columns, or (P2) hi and lo over the 32
-            // columns of S that were read just before.
+            // columns of S they came from.
             float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-            const float2 neg_m = make_float2(-m, -m), minus1 = make_float2(-1.f, -1.f);
+            const float2 neg_m = make_float2(-m, -m);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 uint32_t ph[16], pl[P2 ? 16 : 1];
-                if (!__any_sync(0xffffffffu, seen[c] != 0)) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        ph[j] = 0u;
-                        if constexpr (P2) pl[j] = 0u;
-                    }
-                } else {
-                    float s[32];
-                    fa_ld32(lanes + kColS + 32 * c, s);
+                float* sc = s + (BOUNDED ? 0 : 32 * c);
+                if (BOUNDED && (alive >> c & 1)) {
+                    fa_ld32(lanes + kColS + 32 * c, sc);
                     fa_wait_ld();
-                    if (BOUNDED || (CAP == kCapNone && !BIAS)) {
-                        const bool whole = __all_sync(0xffffffffu, seen[c] == 0xffffffffu);
-                        apply_rules<CAP, BIAS>(s, a.rule.cap, slope, (float)(pos - k0 - 32 * c), whole ? 0xffffffffu : seen[c]);
-                    }
+                }
+                if (BOUNDED && !P2 && c == 3) s_is_read(b, lane);
+                if (alive >> c & 1) {
+                    if (BOUNDED) rules<CAP, BIAS>(sc, a.rule.cap, slope, pos - k0 - 32 * c, lo - k0 - 32 * c, hi - k0 - 32 * c, whole);
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        const float2 x = __fadd2_rn(make_float2(s[2 * j], s[2 * j + 1]), neg_m);
+                        float2 x = make_float2(sc[2 * j], sc[2 * j + 1]);
+                        if (!BOUNDED || BIAS) x = __fadd2_rn(x, neg_m);
                         const float2 e = make_float2(score_exp2(x.x), score_exp2(x.y));
                         sum[j & 1] = __fadd2_rn(sum[j & 1], e);
                         ph[j] = pack_bf16x2(e.x, e.y);
@@ -260,6 +352,12 @@ __global__ void __launch_bounds__(kThreadsP, 2) score_prompt_kernel(ScorePromptA
                             const float2 d = __ffma2_rn(make_float2(bf16lo(ph[j]), bf16hi(ph[j])), minus1, e);
                             pl[j] = pack_bf16x2(d.x, d.y);
                         }
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        ph[j] = 0u;
+                        if constexpr (P2) pl[j] = 0u;
                     }
                 }
                 if constexpr (P2) {
@@ -271,61 +369,43 @@ __global__ void __launch_bounds__(kThreadsP, 2) score_prompt_kernel(ScorePromptA
             }
             l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
             wait_st();
-            if (k0 < lo_most || k0 + KT - 1 > hi_least) {
-                // Some row does not see some key: thread = key, its V row cleaned in shared memory.
+            if (!whole) {  // some row does not see some key: a V row a thread, cleaned in shared memory
                 ok = __all_sync(0xffffffffu, mbar_wait(&b->vfull[i % kSlots], (i / kSlots) & 1));
                 if (!ok) break;
-                uint4* v = reinterpret_cast<uint4*>(sm + kOffV + (i % kSlots) * kTile + tid * 128);
-                const bool gone = k0 + tid >= end;
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    uint4 w = gone ? make_uint4(0u, 0u, 0u, 0u) : v[c ^ (tid & 7)];
-                    const bool bad = drop_not_finite(w.x) | drop_not_finite(w.y) | drop_not_finite(w.z) | drop_not_finite(w.w);
-                    if (gone || bad) v[c ^ (tid & 7)] = w;
-                    if (bad) s_bad = 1;
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                clean_v(sm + kOffV + (i % kSlots) * kTile, tid, k0 + tid >= end, &s_bad);
             }
             fa_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&b->pfull);
-        }
-        // O / l to the output (zeros for rows that see nothing).
-        if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&b->odone, (n - 1) & 1));
-        if (!ok && lane == 0) set_error(a.err, DEV_ERR_TIMEOUT);
-        asm volatile("bar.sync 1, 128;" ::: "memory");  // s_bad of every softmax warp (all come here)
-        const bool bad = *const_cast<volatile int*>(&s_bad) != 0;
-        if (ok) {
+            if (++kt < n) continue;
+            // The head's end: O / l to the output. P V done also means that every warp's s_bad is seen
+            // (they wrote it before their arrivals on pfull).
+            ok = __all_sync(0xffffffffu, mbar_wait(&b->odone, i & 1));
+            if (!ok) break;
             fa_after();
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            const long long at = (long long)(row0 + tid) * a.ld + head * kHeadDim;
+            const bool bad = *const_cast<volatile int*>(&s_bad) != 0;
+            const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 float o[32];
-                if (n > 0) {
-                    fa_ld32(lanes + kColO + 32 * c, o);
-                    fa_wait_ld();
-                }
+                fa_ld32(lanes + kColO + 32 * c, o);
+                fa_wait_ld();
                 if (there) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) o[j] = n > 0 ? o[j] * inv : 0.f;
-                    if (bad) add_not_finite(a, kv_row, kv_x + 32 * c, lo, hi, o);
-                    if constexpr (P2) {
-                        float4* out = reinterpret_cast<float4*>(static_cast<float*>(a.out) + at + 32 * c);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) out[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-                    } else {
-                        uint4* out = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + at + 32 * c);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            out[j] = make_uint4(pack_bf16x2(o[8 * j], o[8 * j + 1]), pack_bf16x2(o[8 * j + 2], o[8 * j + 3]),
-                                                pack_bf16x2(o[8 * j + 4], o[8 * j + 5]), pack_bf16x2(o[8 * j + 6], o[8 * j + 7]));
-                    }
+                    for (int j = 0; j < 32; ++j) o[j] *= inv;
+                    if (bad) add_not_finite(a, kv_row(head), kv_x(head) + 32 * c, lo, hi, o);
+                    store_half<P2>(a, row0 + r, head, c, o);
                 }
                 __syncwarp();
             }
+            fa_before();  // O is read before the next head's first P V (through pfull)
+            kt = 0;
+            ++head;
         }
-    } else if (warp == kMmaW && lane == 0) {
+        if (!ok && lane == 0) set_error(a.err, DEV_ERR_TIMEOUT);
+    } else {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
+      if (warp == kMmaW && lane == 0) {
         // ---- MMA issuer ------------------------------------------------------------------------
         auto issue_s = [&](int i) {
             fa_after();
@@ -337,6 +417,7 @@ __global__ void __launch_bounds__(kThreadsP, 2) score_prompt_kernel(ScorePromptA
             }
             fa_commit(&b->sfull);
             fa_commit(&b->kempty[i % kSlots]);
+            if (i % n == n - 1) fa_commit(&b->qfree);  // the head's last use of Q
         };
         auto issue_pv = [&](int i) {
             fa_after();
@@ -344,50 +425,56 @@ __global__ void __launch_bounds__(kThreadsP, 2) score_prompt_kernel(ScorePromptA
 #pragma unroll
             for (int k = 0; k < 8; ++k) {  // 128 keys, 16 a step: 8 columns of P, 16 rows (2048 bytes) of V
                 const uint32_t p = P2 ? tmem + kColS + 32 * (k >> 1) + 8 * (k & 1) : tmem + kColP + 8 * k;
-                fa_mma_ts(tmem + kColO, p, dv + 128 * k, kIdescPV, (i || k) ? 1u : 0u);
+                fa_mma_ts(tmem + kColO, p, dv + 128 * k, kIdescPV, (i % n || k) ? 1u : 0u);
                 if (P2) fa_mma_ts(tmem + kColO, p + 16, dv + 128 * k, kIdescPV, 1u);
             }
             fa_commit(&b->odone);
             fa_commit(&b->vempty[i % kSlots]);
         };
-        auto k_there = [&](int i) { return mbar_wait(&b->kfull[i % kSlots], (i / kSlots) & 1); };
-        bool ok = n == 0 || (mbar_wait(&b->qready, 0) && k_there(0));
-        if (ok && n > 0) issue_s(0);
-        for (int i = 0; i < n && ok; ++i) {
-            ok = mbar_wait(&b->pfull, i & 1);
-            if (!P2 && ok && i + 1 < n && (ok = k_there(i + 1))) issue_s(i + 1);
-            if (ok && (ok = mbar_wait(&b->vfull[i % kSlots], (i / kSlots) & 1))) issue_pv(i);
-            // P lies over S: the next scores wait for P V.
-            if (P2 && ok && i + 1 < n && (ok = k_there(i + 1) && mbar_wait(&b->odone, i & 1))) issue_s(i + 1);
+        auto there_for_s = [&](int i) {
+            return mbar_wait(&b->kfull[i % kSlots], (i / kSlots) & 1) && mbar_wait(&b->qready, (i / n) & 1);
+        };
+        bool ok = items == 0 || there_for_s(0);
+        if (ok && items > 0) issue_s(0);
+        for (int i = 0; i < items && ok; ++i) {
+            // The next scores as soon as the softmax holds these in registers (P2: P lies over S, so
+            // after P V).
+            if (!P2 && i + 1 < items && (ok = there_for_s(i + 1) && mbar_wait(&b->sfree, i & 1))) issue_s(i + 1);
+            if (ok && (ok = mbar_wait(&b->pfull, i & 1) && mbar_wait(&b->vfull[i % kSlots], (i / kSlots) & 1))) issue_pv(i);
+            if (P2 && ok && i + 1 < items && (ok = there_for_s(i + 1) && mbar_wait(&b->odone, i & 1))) issue_s(i + 1);
         }
         if (!ok) set_error(a.err, DEV_ERR_TIMEOUT);
-    } else if (warp == kLoadW && lane == 0 && n > 0) {
+    } else if (warp == kLoadW && lane == 0) {
         // ---- Q, K and V producer -----------------------------------------------------------------
-        mbar_arrive_expect_tx(&b->qready, 2 * kTile);
-        fa_tma(base, &tm_qh, head * kHeadDim, row0, &b->qready);
-        fa_tma(base + kTile, &tm_ql, head * kHeadDim, row0, &b->qready);
         bool ok = true;
-        for (int i = 0; i < n && ok; ++i) {
-            const int slot = i % kSlots, y = kv_row + first + i * KT;
-            if (i >= kSlots) ok = mbar_wait(&b->kempty[slot], ((i / kSlots) & 1) ^ 1);
-            if (!ok) break;
+        for (int i = 0, kt = 0, hh = 0; i < items && ok; ++i) {
+            const int slot = i % kSlots, head = head0 + hh, y = kv_row(head) + first + (n - 1 - kt) * KT;
+            if (kt == 0) {
+                if (hh > 0 && !(ok = mbar_wait(&b->qfree, (hh - 1) & 1))) break;
+                mbar_arrive_expect_tx(&b->qready, 2 * kTile);
+                fa_tma(base, &tm_qh, head * kHeadDim, row0, &b->qready);
+                fa_tma(base + kTile, &tm_ql, head * kHeadDim, row0, &b->qready);
+                s_q_issued = hh + 1;
+            }
+            if (i >= kSlots && !(ok = mbar_wait(&b->kempty[slot], ((i / kSlots) & 1) ^ 1))) break;
             mbar_arrive_expect_tx(&b->kfull[slot], kTile);
-            fa_tma(base + kOffK + slot * kTile, &tm_k, kv_x, y, &b->kfull[slot]);
+            fa_tma(base + kOffK + slot * kTile, &tm_k, kv_x(head), y, &b->kfull[slot]);
             s_k_issued = i + 1;
-            if (i >= kSlots) ok = mbar_wait(&b->vempty[slot], ((i / kSlots) & 1) ^ 1);
-            if (!ok) break;
+            if (i >= kSlots && !(ok = mbar_wait(&b->vempty[slot], ((i / kSlots) & 1) ^ 1))) break;
             mbar_arrive_expect_tx(&b->vfull[slot], kTile);
-            fa_tma(base + kOffV + slot * kTile, &tm_v, kv_x, y, &b->vfull[slot]);
+            fa_tma(base + kOffV + slot * kTile, &tm_v, kv_x(head), y, &b->vfull[slot]);
             s_v_issued = i + 1;
+            if (++kt == n) kt = 0, ++hh;
         }
         if (!ok) set_error(a.err, DEV_ERR_TIMEOUT);
+      }
     }
     fa_before();
     __syncthreads();
-    if (tid == 0 && n > 0) {
+    if (tid == 0) {
         // The last copies into each slot land before the shared memory goes (a completed phase returns
         // at once).
-        mbar_wait(&b->qready, 0);
+        if (s_q_issued > 0) mbar_wait(&b->qready, (s_q_issued - 1) & 1);
         for (int i = max(0, s_k_issued - kSlots); i < s_k_issued; ++i) mbar_wait(&b->kfull[i % kSlots], (i / kSlots) & 1);
         for (int i = max(0, s_v_issued - kSlots); i < s_v_issued; ++i) mbar_wait(&b->vfull[i % kSlots], (i / kSlots) & 1);
     }
@@ -401,7 +488,7 @@ template <int CAP, bool BOUNDED, bool P2>
 void launch_bias(const ScorePromptArgs& a, const CUtensorMap* m, cudaStream_t s) {
     auto go = [&](auto kernel) {
         set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), kSmemP);
-        launch_k(kernel, dim3((unsigned)(a.n_tiles * a.heads)), dim3(kThreadsP), kSmemP, s, a, m[0], m[1], m[2], m[3]);
+        launch_k(kernel, dim3((unsigned)(a.n_tiles * (a.heads / a.heads_per_cta))), dim3(kThreadsP), kSmemP, s, a, m[0], m[1], m[2], m[3]);
     };
     if (a.rule.slopes) go(score_prompt_kernel<CAP, BOUNDED, true, P2>);
     else go(score_prompt_kernel<CAP, BOUNDED, false, P2>);

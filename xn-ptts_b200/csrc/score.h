@@ -83,7 +83,7 @@ struct ScoreCoreArgs {
 void launch_score_core(const ScoreCoreArgs& a, bool cache_bf16, cudaStream_t s);
 
 // How the matrix-product kernels cap scores: not, by the fast form (bf16 outputs, caps up to
-// kScoreFastCap; q is then scaled by 2 log2(e) / (8 cap)) or by tanhf (q scaled by log2(e) / 8, as
+// kScoreFastCap; q is then scaled by 1 / (8 cap)) or by tanhf (q scaled by log2(e) / 8, as
 // without a cap).
 enum { kCapNone = 0, kCapFast = 1, kCapExact = 2 };
 constexpr float kScoreFastCap = 128.f;
@@ -92,7 +92,7 @@ inline int score_cap_mode(float cap, bool out_f32) {
 }
 inline float score_q_scale(float cap, bool out_f32) {
     constexpr float log2e = 1.4426950408889634f;
-    return score_cap_mode(cap, out_f32) == kCapFast ? 0.25f * log2e / cap : 0.125f * log2e;
+    return score_cap_mode(cap, out_f32) == kCapFast ? 0.125f / cap : 0.125f * log2e;
 }
 
 // Few rows over a whole cache on mma.sync, bf16 caches (attn_rows.cu): blocks of up to
@@ -135,6 +135,7 @@ struct ScorePromptArgs {
     ScoreRule rule;
     const int2* tiles;
     int n_tiles;
+    int heads_per_cta;    // 1, 2, 4 or 8
     uint32_t* err;
 };
 bool launch_score_prompt(const ScorePromptArgs& a, cudaStream_t s);

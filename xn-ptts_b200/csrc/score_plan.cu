@@ -3,8 +3,7 @@
 // split kernels. The ordinary attention op plans and appends in two launches.
 //
 // RoPE and append as in rope_append.cu (rope.rs:81-95, complete_kv at transformer.rs:84-91): one
-// CTA per row, one warp per head, a lane per pair, so the angle's sine and cosine are computed
-// once per warp rather than once per head.
+// warp per row, whose lanes compute the 32 pairs' sines and cosines once for all heads.
 //
 // Bound by memory for prompts (per row (H + 2 KVH) x 64 inputs read, H x 64 x 2 cache elements and
 // the q planes written) and by launch latency for single tokens.
@@ -26,6 +25,19 @@ __device__ __forceinline__ int seq_of(const ScorePlanArgs& a, int r) {
         const int mid = (lo + hi + 1) >> 1;
         if (offsets[mid] <= r) lo = mid;
         else hi = mid - 1;
+    }
+    return lo;
+}
+
+// The same by a warp for one row: 31 probes a step.
+__device__ __forceinline__ int seq_of_warp(const ScorePlanArgs& a, int r, int lane) {
+    if (a.n_seq == a.n_rows) return r;
+    int lo = 0, hi = a.n_seq - 1;  // offsets[lo] <= r, offsets[hi + 1] > r
+    while (lo < hi) {
+        const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step;
+        const int below = __popc(__ballot_sync(0xffffffffu, at <= hi && a.row_offsets[min(at, hi)] <= r));
+        lo += below * step;
+        hi = min(hi, lo + step - 1);
     }
     return lo;
 }
@@ -114,105 +126,151 @@ __device__ void plan_units(const ScorePlanArgs& a) {
     }
 }
 
-template <typename Tin>
-__device__ __forceinline__ float2 load_pair(const void* p, long long pair);
-template <>
-__device__ __forceinline__ float2 load_pair<float>(const void* p, long long pair) {
-    return static_cast<const float2*>(p)[pair];
+// 16 bytes of an input row as floats: 8 bf16 or 4 f32.
+__device__ __forceinline__ void load_in(const __nv_bfloat16* p, float* x) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    x[0] = bf16lo(u.x), x[1] = bf16hi(u.x), x[2] = bf16lo(u.y), x[3] = bf16hi(u.y);
+    x[4] = bf16lo(u.z), x[5] = bf16hi(u.z), x[6] = bf16lo(u.w), x[7] = bf16hi(u.w);
 }
-template <>
-__device__ __forceinline__ float2 load_pair<__nv_bfloat16>(const void* p, long long pair) {
-    const uint32_t u = static_cast<const uint32_t*>(p)[pair];
-    return make_float2(bf16lo(u), bf16hi(u));
+__device__ __forceinline__ void load_in(const float* p, float* x) {
+    const float4 u = *reinterpret_cast<const float4*>(p);
+    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
 }
-__device__ __forceinline__ void store_pair(float* p, float2 v) { *reinterpret_cast<float2*>(p) = v; }
-__device__ __forceinline__ void store_pair(__nv_bfloat16* p, float2 v) {
-    *reinterpret_cast<uint32_t*>(p) = pack_bf16x2(v.x, v.y);
+template <int E>
+__device__ __forceinline__ void store_out(float* p, const float* x) {
+#pragma unroll
+    for (int i = 0; i < E; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+}
+template <int E>
+__device__ __forceinline__ void store_out(__nv_bfloat16* p, const float* x) {
+    uint32_t w[E / 2];
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+    if constexpr (E == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
 }
 
 template <typename Tin, typename T>
 __global__ void __launch_bounds__(kPlanThreads) score_plan_kernel(ScorePlanArgs a) {
-    __shared__ int s_parent[kTreeNodes];
-    __shared__ int s_pos;
     grid_dep_wait();
     grid_dep_launch();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int r = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int block = blockIdx.x;
     if (a.n_units > 0) {
-        if (r == 0) {
+        if (block == 0) {
             plan_units(a);
             return;
         }
-        r -= 1;
+        block -= 1;
     }
-    const int sq = seq_of(a, r), row0 = a.row_offsets[sq];
+    // A warp per row.
+    const int r = block * kPlanWarps + warp;
+    if (r >= a.n_rows) return;
+    const int sq = seq_of_warp(a, r, lane), row0 = a.row_offsets[sq];
     const int rows = a.row_offsets[sq + 1] - row0, sid = a.seq_stream[sq];
     const bool known = sid >= 0 && sid < a.num_streams;
     const int base = known ? a.lengths[sid] : 0;
     const int node = r - row0, slot = base + node;
     bool good = known && base >= 0 && slot < a.capacity;
-    if (!good && tid == 0) set_error(a.err, known ? DEV_ERR_CAPACITY : DEV_ERR_BOUNDS);
-    int pos = slot;
-    if (a.parents) {  // one bad parent refuses the whole tree: every node's CTA sees it
-        const int p = tid < rows ? a.parents[row0 + tid] : -1;
-        if (tid < kTreeNodes) s_parent[tid] = p;
-        if (__syncthreads_or(tid < rows && (p < -1 || p >= tid))) {
-            if (tid == 0) set_error(a.err, DEV_ERR_BOUNDS);
+    if (!good && lane == 0) set_error(a.err, known ? DEV_ERR_CAPACITY : DEV_ERR_BOUNDS);
+    int pos = slot, lo = 0, hi = -1;
+    if (good) row_span(a, r, base, row0, rows, lo, hi);
+    unsigned long long seen = 0;
+    if (a.parents) {
+        // Lane i holds the parents of nodes i and 32 + i. One bad parent refuses the whole tree: every
+        // row's warp sees it.
+        const int p0 = lane < rows ? a.parents[row0 + lane] : -1;
+        const int p1 = lane + 32 < rows ? a.parents[row0 + lane + 32] : -1;
+        if (__any_sync(0xffffffffu, p0 < -1 || p0 >= lane || p1 < -1 || p1 >= lane + 32)) {
+            if (lane == 0) set_error(a.err, DEV_ERR_BOUNDS);
             good = false;
+            lo = 0, hi = -1;
         }
-        if (good && tid == 0) {
-            int depth = 0;
-            for (int i = s_parent[node]; i >= 0; i = s_parent[i]) ++depth;
-            s_pos = base + depth;
+        // The path to the root: parents fall, so it ends; the node and its ancestors, a bit each.
+        int depth = 0;
+        for (int i = node; good && i >= 0;) {
+            seen |= 1ull << i;
+            const int up = __shfl_sync(0xffffffffu, i < 32 ? p0 : p1, i & 31);
+            depth += up >= 0;
+            i = up;
         }
-        __syncthreads();
-        if (good) pos = s_pos;
+        pos = base + depth;
+        // Of these, the ones at positions from `lo` on: positions fall by one from node to parent,
+        // so drop the lowest bits (the roots' end) of those before it.
+        for (int drop = lo - base; drop > 0 && seen; --drop) seen &= seen - 1;
+        if (hi < 0) seen = 0;
     }
-    if (tid == 0) {
-        int lo = 0, hi = -1;
-        if (good) row_span(a, r, base, row0, rows, lo, hi);
+    if (lane == 0) {
         a.rows.stream[r] = good ? sid : -1;
         a.rows.pos[r] = pos;
         a.rows.lo[r] = lo;
         a.rows.hi[r] = hi;
         if (a.parents) {
-            // Itself and its ancestors, those at positions from `lo` on (a path's positions
-            // fall by one from node to parent).
-            unsigned long long seen = 0;
-            if (good && hi >= 0)
-                for (int i = node, at = pos; i >= 0 && at >= lo; i = s_parent[i], --at) seen |= 1ull << i;
             a.rows.base[r] = base;
             a.rows.row0[r] = row0;
             a.rows.lineage[r] = seen;
         }
     }
-    // RoPE and append: lane = pair, warps over the heads of q, k and v.
-    float sn = 0.f, cs = 1.f;
-    if (a.rotate) sincosf((float)pos * a.inv_freq[lane], &sn, &cs);
-    const int group = a.heads / a.kv_heads;
-    for (int h = warp; h < a.heads + 2 * a.kv_heads; h += kPlanWarps) {
-        const int part = h < a.heads ? 0 : (h < a.heads + a.kv_heads ? 1 : 2);  // q, k, v
-        const int hh = part == 0 ? h : h - a.heads - (part - 1) * a.kv_heads;
-        const long long at = ((long long)r * (part == 0 ? a.heads : a.kv_heads) + hh) * (kHeadDim / 2) + lane;
-        float2 x = load_pair<Tin>(part == 0 ? a.q : (part == 1 ? a.k : a.v), at);
-        if (part < 2 && a.rotate) {
-            const float y0 = __fsub_rn(__fmul_rn(x.x, cs), __fmul_rn(x.y, sn));
-            const float y1 = __fadd_rn(__fmul_rn(x.x, sn), __fmul_rn(x.y, cs));
-            x = make_float2(y0, y1);
+    // RoPE and append, 16 bytes of input a lane: E dims of one of the HS heads a warp takes at a time.
+    // Lane i turns pair i; a lane's own pairs' factors come from there.
+    constexpr int E = 16 / (int)sizeof(Tin), HS = 32 * E / kHeadDim;
+    float cs[E / 2], sn[E / 2];
+    if (a.rotate) {
+        float s, c;
+        sincosf((float)pos * a.inv_freq[lane], &s, &c);
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) {
+            const int pair = lane % (kHeadDim / E) * (E / 2) + i;
+            cs[i] = __shfl_sync(0xffffffffu, c, pair);
+            sn[i] = __shfl_sync(0xffffffffu, s, pair);
         }
-        if (part == 0) {
-            if (a.q_hi) {
-                const float y0 = x.x * a.q_scale, y1 = x.y * a.q_scale;
-                const uint32_t hi = pack_bf16x2(y0, y1);
-                reinterpret_cast<uint32_t*>(a.q_hi)[at] = hi;
-                reinterpret_cast<uint32_t*>(a.q_lo)[at] = pack_bf16x2(y0 - bf16lo(hi), y1 - bf16hi(hi));
-            } else {
-                store_pair(a.q_out + 2 * at, x);
+    }
+    auto rotate = [&](float* x) {
+        if (!a.rotate) return;
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) {
+            const float x0 = x[2 * i], x1 = x[2 * i + 1];
+            x[2 * i] = __fsub_rn(__fmul_rn(x0, cs[i]), __fmul_rn(x1, sn[i]));
+            x[2 * i + 1] = __fadd_rn(__fmul_rn(x0, sn[i]), __fmul_rn(x1, cs[i]));
+        }
+    };
+    const int mine = lane / (kHeadDim / E), dim = lane % (kHeadDim / E) * E;  // of a step's heads; first dim
+    const Tin* q = static_cast<const Tin*>(a.q) + (long long)r * a.heads * kHeadDim + dim;
+#pragma unroll 2
+    for (int h = mine; h < a.heads; h += HS) {
+        const long long at = ((long long)r * a.heads + h) * kHeadDim + dim;
+        float x[E];
+        load_in(q + h * kHeadDim, x);
+        rotate(x);
+        if (a.q_hi) {
+            float lo[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                x[i] *= a.q_scale;
+                lo[i] = x[i] - __bfloat162float(__float2bfloat16_rn(x[i]));
             }
-        } else if (good) {
-            T* cache = static_cast<T*>(part == 1 ? a.k_cache : a.v_cache);
-            for (int rep = 0; rep < group; ++rep)
-                store_pair(cache + kv_offset(sid, slot, hh * group + rep, a.num_streams, a.capacity) + 2 * lane, x);
+            store_out<E>(a.q_hi + at, x);
+            store_out<E>(a.q_lo + at, lo);
+        } else {
+            store_out<E>(a.q_out + at, x);
+        }
+    }
+    if (!good) return;
+    const int group = a.heads / a.kv_heads;
+    const Tin* k = static_cast<const Tin*>(a.k) + (long long)r * a.kv_heads * kHeadDim + dim;
+    const Tin* v = static_cast<const Tin*>(a.v) + (long long)r * a.kv_heads * kHeadDim + dim;
+    T* kc = static_cast<T*>(a.k_cache) + dim;
+    T* vc = static_cast<T*>(a.v_cache) + dim;
+#pragma unroll 2
+    for (int h = mine; h < a.kv_heads; h += HS) {
+        float x[E], y[E];
+        load_in(k + h * kHeadDim, x);
+        load_in(v + h * kHeadDim, y);
+        rotate(x);
+        for (int rep = 0; rep < group; ++rep) {
+            const long long to = kv_offset(sid, slot, h * group + rep, a.num_streams, a.capacity);
+            store_out<E>(kc + to, x);
+            store_out<E>(vc + to, y);
         }
     }
 }
@@ -220,7 +278,7 @@ __global__ void __launch_bounds__(kPlanThreads) score_plan_kernel(ScorePlanArgs 
 }  // namespace
 
 void launch_score_plan(const ScorePlanArgs& a, bool in_bf16, bool cache_bf16, cudaStream_t s) {
-    const dim3 grid(a.n_rows + (a.n_units > 0 ? 1 : 0)), block(kPlanThreads);
+    const dim3 grid((a.n_rows + kPlanWarps - 1) / kPlanWarps + (a.n_units > 0 ? 1 : 0)), block(kPlanThreads);
     if (in_bf16 && cache_bf16) launch_k(score_plan_kernel<__nv_bfloat16, __nv_bfloat16>, grid, block, 0, s, a);
     else if (in_bf16) launch_k(score_plan_kernel<__nv_bfloat16, float>, grid, block, 0, s, a);
     else if (cache_bf16) launch_k(score_plan_kernel<float, __nv_bfloat16>, grid, block, 0, s, a);
