@@ -400,8 +400,13 @@ class KvState:
         the stream grows by their number (ptts_b200_kv_accept)."""
         if len(nodes) != len(streams):
             raise PttsError(ERR_ARG, "one path per stream")
-        st, flat = _i32(streams), _i32([x for path in nodes for x in path])
-        counts = _i32([len(path) for path in nodes])
+        st, counts = _i32(streams), np.fromiter(map(len, nodes), np.int32, len(nodes))
+        try:  # node indexes are below 64: lists of them flatten fastest as bytes
+            if not set(map(type, nodes)) <= {list, tuple}:
+                raise ValueError
+            flat = np.frombuffer(b"".join(map(bytes, nodes)), np.uint8).astype(np.int32)
+        except (ValueError, TypeError):  # other sequences, or indexes that the library will refuse
+            flat = _i32([x for path in nodes for x in path])
         _check(lib().ptts_b200_kv_accept(self._h, _ip(st), _ip(counts), _ip(flat), len(st),
                                          _stream_of(self.device, stream)))
 

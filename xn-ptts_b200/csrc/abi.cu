@@ -625,15 +625,12 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
     const int most = *std::max_element(rows_host, rows_host + n_seq);
     const bool tokens = !tree && n_rows == n_seq, few = !tokens && cache_bf16 && most <= kTreeNodes;
     const bool prompt = !tokens && cache_bf16 && !few, out_bf16 = out_dtype == PTTS_B200_BF16;
-    int block = 0, grid = sm_count(kv->device);
+    int grid = sm_count(kv->device);
     std::vector<int2> blocks;
     if (prompt) blocks = make_tiles(offsets, streams_host, kv->h_len);
     if (few) {
-        block = score_rows_block(most);
-        grid = score_rows_grid(block, kv->heads, grid);
-        for (int i = 0; i < n_seq; ++i)
-            for (int r = offsets[i]; r < offsets[i + 1]; r += block)
-                blocks.push_back(make_int2(r, std::min(block, offsets[i + 1] - r)));
+        grid = score_rows_grid(out_bf16, kv->heads, grid);
+        for (int i = 0; i < n_seq; ++i) blocks.push_back(make_int2(offsets[i], rows_host[i]));
     }
     std::vector<int32_t> packed(streams_host, streams_host + n_seq);
     packed.insert(packed.end(), offsets.begin(), offsets.end());
@@ -738,9 +735,11 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
         a.prefix = p.prefix;
         a.unit_lo = p.unit_lo;
         a.cta_first = p.cta_first;
-        a.part = static_cast<float*>(kv->part.need(sizeof(float) * score_rows_part_floats(block, kv->heads, grid)));
+        a.n_rows = n_rows;
+        a.most_rows = most;
+        a.part = static_cast<float*>(kv->part.need(sizeof(float) * score_rows_part_floats(kv->heads, grid)));
         a.err = p.err;
-        require(launch_score_rows(a, block, grid, s), PTTS_B200_ERR_CUDA,
+        require(launch_score_rows(a, grid, s), PTTS_B200_ERR_CUDA,
                 "could not describe the cache's tensors (cuTensorMapEncodeTiled)");
         check_launch();
         return;

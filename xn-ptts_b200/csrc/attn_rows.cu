@@ -1,432 +1,563 @@
 // Attention with score rules for a few rows per stream over its whole cache (drafted trees, short
-// prompts on long caches), bf16 caches: blocks of up to 64 rows of one sequence, split over the keys.
+// prompts on long caches), bf16 caches: blocks of up to 64 rows of one sequence, split over the keys,
+// on tcgen05 with the keys as the tall side.
 //
-// Bound by HBM: a block's keys and values are read once for all its rows, so the time is that of
-// the cache bytes as long as the matrix products keep up. Per key and head 256 bytes arrive (about
-// 11 cycles of an SM's share of HBM); 64 rows need 64 x 64 x 3 multiply-adds there (q as a bf16
-// hi/lo pair, P as one bf16), which mma.sync does within that time, so the rows stay in registers
-// as mma fragments and the 128-row tiles of tcgen05, half or three quarters empty here, are left
-// to the prompts (attn_score_prompt.cu).
+// Bound by HBM: a block's keys and values are read once for all its rows. Per key and head 256 bytes
+// arrive, about 11 cycles of an SM's share of HBM. With rows as an MMA's M side, half or more of its
+// 128 rows would be empty, and mma.sync (2048 flops a cycle and SM) needs those 11 cycles for 64 rows
+// alone; so keys are M and rows are N, which a call pays for in steps of 16:
+//   S^T = K Q^T     128 keys x N rows, q as a bf16 hi/lo pair: 2 x 2 N cycles
+//   O^T += V^T P^T  (64 dims and a row of ones) x N rows over 128 keys: 4 N cycles; the ones give the
+//                   rows' sums of P beside their products, in lane 64
+// At N = 64 that is 4 cycles a key, and the softmax 4 (64 exp2 at 16 a cycle), side by side.
 //
-// Work split as in attn_decode.cu: the blocks' keys lie end to end and every CTA takes an equal
-// range, cut at no tile boundary. One producer lane copies chunks of 32 keys by TMA (one 3-D copy
-// each for K and V: 64 dims x 32 keys x the CTA's heads, 128-byte swizzle, so that ldmatrix reads
-// are free of bank conflicts) into a ring of 192 KB. The consumer warps each own (a head, 16 or 32
-// rows): S = Q K^T in f32 fragments, rules and mask, an online softmax whose maximum is raised only
-// when a score passes it by 2^8, then O += P V from the S fragments' registers. A block inside one
-// CTA's range is written at once; the pieces of a cut block leave (max, sum, acc) records that a
-// second kernel joins, one warp per row and head: 64 rows x 8 heads are too many for the warp that
-// finishes last.
+// Work split as in attn_decode.cu: the blocks' keys lie end to end and every CTA takes an equal range,
+// for two heads (f32 outputs: one), each head a pipeline of its own:
+//   warps 0-3, 4-7  a thread per key (TMEM lane) of the head's 128-key item, its scores against all rows
+//                   in registers: rules, mask, exp2 against the rows' maxima in shared memory, P^T as
+//                   bf16 into shared memory (key by key, rows adjacent: the MMA's B operand). No sums and
+//                   no maxima cross threads, unless a score passes its row's maximum by 2^8: then the
+//                   128 threads take the item's maxima (an integer reduction per row) and rescale O.
+//                   Caps up to kScoreBoundedCap need no maxima at all (see attn_score_prompt.cu).
+//   warps 8, 9      one lane each issues a head's MMAs; the next item's S starts when this one's scores
+//                   are in registers.
+//   warp 10         one lane copies the heads' Q tiles and K and V items by TMA, two slots each.
+// A block inside one CTA's range is written at once; the pieces of a cut block leave (max, sum, acc)
+// records that a second kernel joins, one warp per row and head: 64 rows x 8 heads are too many for
+// the warp that finishes last.
 //
-// Shapes: up to 16 rows, 8 heads a CTA and a warp a head; up to 32 the same with two 16-row tiles
-// a warp; up to 64, 4 heads a CTA (half the grid for each half of the heads) and two warps a head.
-//
-// A chunk that some row does not see whole masks scores by select, and takes values that are not
-// finite out of the V fragments, to add them to the rows that do see them (0 x NaN is NaN, and a
-// visible key's weight is positive).
+// f32 outputs hold P as a bf16 hi/lo pair in two tiles; bf16 outputs round P once to bf16, as the output
+// itself is rounded. An item that some row does not see whole has a bit per row in each key's thread, and
+// takes values that are not finite out of the V tile (0 x NaN is NaN); rows that see such a value get it
+// back at the piece's end, from the cache.
 #include "common.cuh"
+#include "fa_tc.cuh"
 #include "score.cuh"
 #include "score.h"
 
 namespace ptts {
 namespace {
 
-constexpr int KC = 32;             // keys per chunk
-constexpr int kRingBytes = 192 * 1024;
-constexpr int kHeadTile = KC * 128;  // one head's K (or V) chunk: 32 keys x 64 bf16
-constexpr int kWarps = 8;
-// Eight consumer warps and a warpgroup of which one lane produces. Two row tiles a warp need about
-// 220 registers; the launch has 168 a thread (12 warps), so the producers give theirs up: 2 x 128 x
-// 232 + 128 x 24 of the launch's 384 x 168.
-constexpr int kThreadsR = (kWarps + 4) * 32;
-constexpr int kRegsLaunch = 168, kRegsConsumer = 232, kRegsProducer = 24;
-static_assert(kWarps * 32 * kRegsConsumer + 128 * kRegsProducer <= kThreadsR * kRegsLaunch, "the split fits the launch");
-constexpr float kRaise = 8.f;
+constexpr int KT = 128;                 // keys per item
+constexpr int NR = kTreeNodes;          // rows per block at most
+constexpr int kTile = KT * 128;         // a K, V, P or ones tile: 128 keys x 64 bf16
+constexpr int kQTile = NR * 128;        // a plane of a head's q
+constexpr int kSlots = 2;
+// 8 softmax warps, 2 MMA issuers, a producer, a spare. The softmax holds 64 scores a thread: its two
+// warpgroups take most of the launch's 384 x 168 registers.
+constexpr int kThreadsR = 12 * 32, kRegsR = 168, kRegsSoft = 232, kRegsRest = 40;
+static_assert(256 * kRegsSoft + 128 * kRegsRest <= kThreadsR * kRegsR, "the split fits the launch");
+constexpr float kRaiseR = 8.f;
 
-// MT 16-row tiles a warp, WPH warps a head.
-template <int MT_, int WPH_>
-struct Shape {
-    static constexpr int MT = MT_, WPH = WPH_;
-    static constexpr int kRows = 16 * MT * WPH;
-    static constexpr int kHeads = kWarps / WPH;  // heads a CTA
-    static constexpr int kStageBytes = 2 * kHeads * kHeadTile;
-    static constexpr int kStages = kRingBytes / kStageBytes;
-    static constexpr int kSmem = 1024 + kRingBytes + kStages * 64 + 2 * kStages * 8;
+// Shared memory of a CTA of HC heads with PT P tiles a head (1024-aligned tiles).
+template <int HC, int PT>
+struct Smem {
+    static constexpr int kQ = 0;                                  // head: hi, lo
+    static constexpr int kK = kQ + HC * 2 * kQTile;               // head, slot
+    static constexpr int kV = kK + HC * kSlots * kTile;
+    static constexpr int kP = kV + HC * kSlots * kTile;           // head, tile
+    static constexpr int kOnes = kP + HC * PT * kTile;            // past every V slot (an MMA's offset is positive)
+    static constexpr int kRows = kOnes + kTile;
+    static constexpr int kBytes = 1024 + kRows + HC * 4096;
 };
-
-struct RowsHdr {
-    int unit, slot, n, flags;  // the chunk's unit, first slot and keys
-    int row0, nrows;           // the unit's rows
+// A head's rows of the block at hand.
+struct HeadRows {
+    float m[NR], shift[NR], scale[NR], pos[NR], sum[NR];
+    int lo[NR], hi[NR], top[NR], has[NR];  // has: the row has a maximum (or sees nothing)
+    unsigned long long lineage[NR];
+    int bad;
 };
-static_assert(sizeof(RowsHdr) <= 64, "a header per stage");
-constexpr int kRFirst = 1, kRLast = 2, kRWhole = 4, kREnd = 8;
-constexpr int kRBegins = 16;  // the block's keys begin in this CTA's range
+static_assert(sizeof(HeadRows) <= 4096 - 512, "rows and barriers of a head");
+// Barriers of a head. Single buffers for S, P, O and Q: item i completes phase i of sfull, sfree, pfull
+// and odone, piece k phase k of qready and qfree; every waiter asks for every phase in turn.
+struct HeadBars {
+    uint64_t kfull[kSlots], kempty[kSlots], vfull[kSlots], vempty[kSlots], qready, qfree, sfull, sfree, pfull, odone;
+};
+static_assert(sizeof(HeadBars) <= 512, "rows and barriers of a head");
 
-__device__ __forceinline__ void ldsm_x4(uint32_t a, uint32_t* r) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(a));
-}
-__device__ __forceinline__ void ldsm_x4_t(uint32_t a, uint32_t* r) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(a));
-}
-__device__ __forceinline__ void mma_bf16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int y, int z, uint64_t* bar, uint64_t policy) {
+constexpr uint32_t kIdescBase = (1u << 4) | (1u << 7) | (1u << 10) | (8u << 24);  // f32 += bf16 x bf16, M = 128
+
+// Whether `v` held in any of a head's 128 softmax threads (named barrier 1 + head): they all come here.
+__device__ __forceinline__ bool head_any(int hl, bool v) {
+    uint32_t any;
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
-        " [%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(y), "r"(z), "r"(smem_u32(bar)), "l"(policy)
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred q, %2, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any)
+        : "r"((uint32_t)v), "r"(1 + hl)
         : "memory");
+    return any != 0;
 }
-// The slots a row sees, for chunks that some row does not see whole.
-struct Sees {
-    int lo, hi, base;
-    unsigned long long lineage;
-    __device__ __forceinline__ bool operator()(int slot) const {
-        return slot >= lo && slot <= hi && (slot < base || (lineage >> (slot - base) & 1));
+// Floats in an order that integers share (NaN below everything).
+__device__ __forceinline__ int ordered(float x) {
+    const int i = __float_as_int(fmaxf(x, kScoreLow));
+    return i ^ ((i >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float unordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
+
+// The CTA's pieces in order, the same walk for every role: block u, its keys s0 .. s1 - 1 of it.
+struct Walk {
+    const ScoreRowsArgs& a;
+    long long start, end;
+    int u;
+    int s0, s1, lo, row0, nrows;
+    bool whole, begins;
+    __device__ Walk(const ScoreRowsArgs& a_, int c, long long total, int G)
+        : a(a_), start(cta_start(c, total, G)), end(cta_start(c + 1, total, G)), u(a_.cta_first[c] - 1) {}
+    __device__ bool next() {
+        if (++u >= a.n_units) return false;
+        const long long pb = a.prefix[u], pe = a.prefix[u + 1];
+        if (pb >= end) return false;
+        s0 = (int)((start > pb ? start : pb) - pb);
+        s1 = (int)((end < pe ? end : pe) - pb);
+        begins = pb >= start;
+        whole = begins && pe <= end;
+        lo = a.unit_lo[u];
+        row0 = a.blocks[u].x;
+        nrows = a.blocks[u].y;
+        return true;
     }
+    __device__ int items() const { return (s1 - s0 + KT - 1) / KT; }
 };
 
-__device__ __forceinline__ Sees sees_of(const ScoreRows& rows, long long row) {
-    Sees s{rows.lo[row], rows.hi[row], 0x7fffffff, 0};
-    if (rows.lineage) s.base = rows.base[row], s.lineage = rows.lineage[row];
-    return s;
+// The values of the piece's keys that are not finite, from the cache, for one dim of the rows that see them.
+template <int N>
+__device__ __forceinline__ void add_not_finite(const ScoreRowsArgs& a, const HeadRows& R, const Walk& w, int base_slot,
+                                               int head, int dim, float* o) {
+    const int sid = max(a.rows.stream[w.row0], 0);
+    const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.v_cache) + kv_offset(sid, w.lo, head, a.num_streams, a.capacity) + dim;
+    for (int j = w.s0; j < w.s1; ++j) {
+        const float x = __bfloat162float(v[(long long)j * kRowWidth]);
+        if (isfinite(x)) continue;
+        const int slot = w.lo + j, node = slot - base_slot;
+#pragma unroll
+        for (int r = 0; r < N; ++r)
+            if (r < w.nrows && slot >= R.lo[r] && slot <= R.hi[r] && (node < 0 || (R.lineage[r] >> node & 1))) o[r] += x;
+    }
 }
 
-template <class S, int CAP, bool P2>
+template <int HC, int CAP, bool BOUNDED, bool P2>
 __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs a, const __grid_constant__ CUtensorMap tm_k,
-                                                                 const __grid_constant__ CUtensorMap tm_v) {
-    constexpr int MT = S::MT;
+                                                                 const __grid_constant__ CUtensorMap tm_v,
+                                                                 const __grid_constant__ CUtensorMap tm_qh,
+                                                                 const __grid_constant__ CUtensorMap tm_ql) {
+    using L = Smem<HC, P2 ? 2 : 1>;
+    constexpr uint32_t kCols = HC * 128;  // per head: S in 64 columns, O in 64
     extern __shared__ unsigned char smem_raw[];
-    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    unsigned char* hdrs = smem + kRingBytes;
-    uint64_t* full = reinterpret_cast<uint64_t*>(hdrs + S::kStages * 64);
-    uint64_t* empty = full + S::kStages;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < S::kStages; ++i) {
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], kWarps);
+    const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    unsigned char* sm = smem_raw + (base - raw);
+    __shared__ uint32_t s_tmem;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    auto rows_of = [&](int hl) { return reinterpret_cast<HeadRows*>(sm + L::kRows + hl * 4096); };
+    auto bars_of = [&](int hl) { return reinterpret_cast<HeadBars*>(sm + L::kRows + hl * 4096 + 4096 - 512); };
+    if (tid < HC) {
+        HeadBars* b = bars_of(tid);
+        for (int i = 0; i < kSlots; ++i) {
+            mbar_init(&b->kfull[i], 1);
+            mbar_init(&b->kempty[i], 1);
+            mbar_init(&b->vfull[i], 1);
+            mbar_init(&b->vempty[i], 1);
         }
+        mbar_init(&b->qready, 1);
+        mbar_init(&b->qfree, 1);
+        mbar_init(&b->sfull, 1);
+        mbar_init(&b->sfree, 4);
+        mbar_init(&b->pfull, 4);
+        mbar_init(&b->odone, 1);
+        rows_of(tid)->bad = 0;
         fence_mbar_init();
     }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(kCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // The ones: dim 0 of every key is 1, the others 0 (swizzled: chunk 0 of key k is at chunk k % 8).
+    for (int i = tid; i < kTile / 16; i += kThreadsR) {
+        const int key = i >> 3, chunk = (i & 7) ^ (key & 7);
+        reinterpret_cast<uint4*>(sm + L::kOnes)[i] = make_uint4(chunk == 0 ? 0x3f80u : 0u, 0u, 0u, 0u);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    fa_before();
     __syncthreads();
+    fa_after();
+    const uint32_t tmem = s_tmem;
     grid_dep_wait();
     grid_dep_launch();
     const long long total = a.prefix[a.n_units];
     const int G = ctas_in_use(total, gridDim.x), c = blockIdx.x;
-    if (c >= G) return;
-    const int head0 = blockIdx.y * S::kHeads;  // this CTA's heads: within one group of 8
+    const int head0 = blockIdx.y * HC;
+    const bool idle = c >= G;
 
-    if (warp >= kWarps) {
-        // ---- producer ------------------------------------------------------------------------
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsProducer));
-        if (warp != kWarps || lane != 0) return;
-        const long long start = cta_start(c, total, G), end = cta_start(c + 1, total, G);
-        const uint64_t pol = policy_evict_first();
-        const int group = head0 / kGroupHeads;
-        int it = 0;
+    if (warp < 4 * HC) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoft));
+        // ---- softmax: thread = key ----------------------------------------------------------------
+        const int hl = warp >> 2, key = tid & 127, head = head0 + hl;
+        HeadRows* R = rows_of(hl);
+        HeadBars* b = bars_of(hl);
+        const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 128 * hl;
+        const bool biased = a.rule.slopes != nullptr;
+        const float slope = biased ? a.rule.slopes[head] * kScoreLog2e : 0.f;
+        unsigned char* pt = sm + L::kP + hl * (P2 ? 2 : 1) * kTile + key * 128;
         bool ok = true;
-        auto stage_free = [&](int k) {
-            if (mbar_wait(&empty[k % S::kStages], ((k / S::kStages) & 1) ^ 1)) return true;
-            set_error(a.err, DEV_ERR_TIMEOUT);
-            return false;
-        };
-        for (int u = a.cta_first[c]; u < a.n_units && ok; ++u) {
-            const long long pb = a.prefix[u], pe = a.prefix[u + 1];
-            if (pb >= end) break;
-            const int s0 = (int)((start > pb ? start : pb) - pb), s1 = (int)((end < pe ? end : pe) - pb);
-            const int2 rows = a.blocks[u];
-            const int sid = max(a.rows.stream[rows.x], 0);  // a refused tree reads slot 0 and sees nothing
-            const int lo = a.unit_lo[u];
-            const int row = (int)(((long long)group * a.num_streams + sid) * a.capacity);
-            const int whole = pb >= start && pe <= end ? kRWhole : 0;
-            for (int p = s0; p < s1; p += KC, ++it) {
-                if (!(ok = stage_free(it))) break;
-                const int st = it % S::kStages;
-                RowsHdr* hd = reinterpret_cast<RowsHdr*>(hdrs + st * 64);
-                hd->unit = u;
-                hd->slot = lo + p;
-                hd->n = min(KC, s1 - p);
-                hd->flags = (p == s0 ? kRFirst : 0) | (p + KC >= s1 ? kRLast : 0) | whole | (pb < start ? 0 : kRBegins);
-                hd->row0 = rows.x;
-                hd->nrows = rows.y;
-                unsigned char* sb = smem + st * S::kStageBytes;
-                mbar_arrive_expect_tx(&full[st], S::kStageBytes);
-                tma_3d(sb, &tm_k, row + lo + p, head0 % kGroupHeads, &full[st], pol);
-                tma_3d(sb + S::kStageBytes / 2, &tm_v, row + lo + p, head0 % kGroupHeads, &full[st], pol);
+        int i = 0;  // items of this CTA so far
+        Walk w(a, idle ? 0 : c, total, G);
+        // A wait that gives up clears `ok`; the head's other warps learn of it at their next barrier,
+        // and all leave there.
+        while (!idle && w.next()) {
+            // The block's rows.
+            const int base_slot = a.rows.lineage ? a.rows.base[w.row0] : 0x7fffffff;
+            if (key < NR) {
+                const bool there = key < w.nrows;
+                const int row = w.row0 + (there ? key : 0);
+                const int lo = there ? a.rows.lo[row] : 0, hi = there ? a.rows.hi[row] : -1, pos = a.rows.pos[row];
+                R->lo[key] = lo;
+                R->hi[key] = hi;
+                R->pos[key] = (float)pos;
+                R->lineage[key] = there && a.rows.lineage ? a.rows.lineage[row] : 0;
+                // BOUNDED: exp2 against the bias of the nearest visible key. Else the row's first scores set m.
+                R->m[key] = BOUNDED ? -slope * (float)max(max(lo - pos, pos - hi), 0) : 0.f;
+                R->has[key] = lo > hi;
             }
-        }
-        if (ok && stage_free(it)) {
-            reinterpret_cast<RowsHdr*>(hdrs + (it % S::kStages) * 64)->flags = kREnd;
-            mbar_arrive(&full[it % S::kStages]);
-            ++it;
-        }
-        // Let every copy in flight land before the CTA's shared memory goes.
-        for (int k = it > S::kStages ? it - S::kStages : 0; k < it; ++k)
-            if (!mbar_wait(&full[k % S::kStages], (k / S::kStages) & 1)) set_error(a.err, DEV_ERR_TIMEOUT);
-        return;
-    }
-
-    // ---- consumers: warp = (head, 16 MT rows) --------------------------------------------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsConsumer));
-    const int hl = warp / S::WPH, head = head0 + hl, rbase = (warp % S::WPH) * 16 * MT;
-    const int g = lane >> 2, t = lane & 3;
-    const float slope = a.rule.slopes ? a.rule.slopes[head] * kScoreLog2e : 0.f;
-    const bool biased = a.rule.slopes != nullptr;
-    uint32_t qh[MT][4][4], ql[MT][4][4];
-    float o[MT][8][4], m[MT][2], l[MT][2], posf[MT][2];
-    int full_lo = 0, full_hi = -1;
-    bool any = false;  // this warp has rows of the block
-    // ldmatrix addresses within a head's tile: K takes 8 keys x 32 dims a time (matrix = dims), V
-    // 16 keys x 16 dims (matrices: keys, then dims).
-    const int k_row = lane & 7, k_chunk = lane >> 3;
-    const int v_row = (lane & 7) + (lane & 8), v_chunk = lane >> 4;
-    for (int it = 0;; ++it) {
-        const int st = it % S::kStages;
-        if (!mbar_wait(&full[st], (it / S::kStages) & 1)) {
-            set_error(a.err, DEV_ERR_TIMEOUT);
-            break;
-        }
-        const RowsHdr hd = *reinterpret_cast<const RowsHdr*>(hdrs + st * 64);
-        if (hd.flags & kREnd) break;
-        if (hd.flags & kRFirst) {
-            any = rbase < hd.nrows;
-            full_lo = 0, full_hi = 0x7fffffff;
+            bool fresh = !BOUNDED;  // some row has no maximum yet
+            if (head_any(hl, !ok)) break;
+            // Rows lane and 32 + lane: what they see, and the slots that every row sees.
+            int full_lo = 0, full_hi = 0x7fffffff, row_lo[2], row_hi[2];
+            unsigned long long row_line[2];
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const int r = rbase + 16 * i + g + 8 * b;
-                    const bool there = r < hd.nrows;
-                    const long long row = hd.row0 + (there ? r : 0);
-                    if (there) {
-                        full_lo = max(full_lo, a.rows.lo[row]);
-                        full_hi = min(full_hi, a.rows.lineage ? min(a.rows.hi[row], a.rows.base[row] - 1) : a.rows.hi[row]);
-                    }
-                    posf[i][b] = biased ? (float)a.rows.pos[row] : 0.f;
-                    m[i][b] = kScoreLow;
-                    l[i][b] = 0.f;
-                    // Rows that are not there have q = 0: finite scores that go nowhere.
-                    const uint32_t* ph = reinterpret_cast<const uint32_t*>(a.q_hi + row * a.ld + head * kHeadDim) + t;
-                    const uint32_t* pl = reinterpret_cast<const uint32_t*>(a.q_lo + row * a.ld + head * kHeadDim) + t;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        qh[i][k][b] = there ? ph[8 * k] : 0u;
-                        qh[i][k][b + 2] = there ? ph[8 * k + 4] : 0u;
-                        ql[i][k][b] = there ? pl[8 * k] : 0u;
-                        ql[i][k][b + 2] = there ? pl[8 * k + 4] : 0u;
-                    }
-                }
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int d = 0; d < 8; ++d)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[i][d][e] = 0.f;
+            for (int x = 0; x < 2; ++x) {
+                const int r = 32 * x + lane;
+                row_lo[x] = R->lo[r], row_hi[x] = R->hi[r], row_line[x] = R->lineage[r];
+                if (r < w.nrows) full_lo = max(full_lo, row_lo[x]), full_hi = min(full_hi, min(row_hi[x], base_slot - 1));
+            }
             full_lo = __reduce_max_sync(0xffffffffu, full_lo);
             full_hi = __reduce_min_sync(0xffffffffu, full_hi);
-        }
-        const unsigned char* kt = smem + st * S::kStageBytes + hl * kHeadTile;
-        const uint32_t ka = smem_u32(kt), va = ka + S::kStageBytes / 2;
-        const bool edge = hd.n < KC || hd.slot < full_lo || hd.slot + KC - 1 > full_hi;
-        if (any) {
-            // S = Q K^T: key 8 n + 2 t (+1) of rows g and g + 8 in s[i][n][0..3].
-            float s[MT][4][4];
+            const int n = w.items(), groups = (w.nrows + 15) / 16;
+            for (int it = 0; it < n; ++it, ++i) {
+                const int slot0 = w.lo + w.s0 + it * KT, slot = slot0 + key;
+                const int count = min(KT, w.s1 - w.s0 - it * KT);  // keys of this item in this CTA's range
+                const bool whole = count == KT && slot0 >= full_lo && slot0 + KT - 1 <= full_hi;
+                // Rows that see this thread's key: key by key, the lanes say it for their two rows.
+                uint32_t seen[2] = {~0u, ~0u};
+                if (!whole) {
+                    const int mine = slot0 + 32 * (warp & 3), keys = w.lo + w.s1;  // this warp's keys; the range's end
+#pragma unroll 4
+                    for (int k = 0; k < 32; ++k) {
+                        const int x = mine + k, node = x - base_slot;
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int n = 0; n < 4; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[i][n][e] = 0.f;
-            // A dims half at a time, its eight accumulators in turn: each mma waits for the one before
-            // it on the same accumulator, 8 (or 4) back.
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                uint32_t kb[4][4];
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    const int key = 8 * n + k_row;
-                    ldsm_x4(ka + key * 128 + (((4 * hf + k_chunk) ^ (key & 7)) << 4), kb[n]);
-                }
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-#pragma unroll
-                    for (int n = 0; n < 4; ++n)
-#pragma unroll
-                        for (int i = 0; i < MT; ++i) mma_bf16(s[i][n], qh[i][2 * hf + k], kb[n][2 * k], kb[n][2 * k + 1]);
-#pragma unroll
-                    for (int n = 0; n < 4; ++n)
-#pragma unroll
-                        for (int i = 0; i < MT; ++i) mma_bf16(s[i][n], ql[i][2 * hf + k], kb[n][2 * k], kb[n][2 * k + 1]);
-                }
-            }
-            // Rules.
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                if (CAP == kCapFast) cap_fast<16>(&s[i][0][0], a.rule.cap);
-                if (CAP == kCapExact) {
-#pragma unroll
-                    for (int n = 0; n < 4; ++n)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[i][n][e] = cap_exact(s[i][n][e], a.rule.cap);
-                }
-                if (biased && !edge) {
-#pragma unroll
-                    for (int n = 0; n < 4; ++n)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float at = (float)(hd.slot + 8 * n + 2 * t + (e & 1));
-                            s[i][n][e] = fmaf(-slope, fabsf(posf[i][e >> 1] - at), s[i][n][e]);
-                        }
-                }
-                if (edge) {
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const int r = rbase + 16 * i + g + 8 * b;
-                        const long long row = hd.row0 + min(r, hd.nrows - 1);
-                        const Sees sees = sees_of(a.rows, row);
-#pragma unroll
-                        for (int n = 0; n < 4; ++n)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int key = 8 * n + 2 * t + e, slot = hd.slot + key;
-                                const bool seen = key < hd.n && sees(slot);
-                                float& x = s[i][n][2 * b + e];
-                                if (biased && seen) {
-                                    const int at = slot < sees.base ? slot : a.rows.pos[a.rows.row0[row] + slot - sees.base];
-                                    x = fmaf(-slope, fabsf(posf[i][b] - (float)at), x);
-                                }
-                                x = seen ? x : -INFINITY;
-                            }
-                    }
-                }
-            }
-            // The running maximum, raised only by more than kRaise.
-            bool raise = false;
-            float mt[MT][2];
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    float x = fmaxf(s[i][0][2 * b], s[i][0][2 * b + 1]);
-#pragma unroll
-                    for (int n = 1; n < 4; ++n) x = fmaxf(x, fmaxf(s[i][n][2 * b], s[i][n][2 * b + 1]));
-                    mt[i][b] = x;
-                    raise |= x > m[i][b] + kRaise;
-                }
-            if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        float x = mt[i][b];
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                        x = fmaxf(x, m[i][b]);
-                        const float f = score_exp2(m[i][b] - x);
-                        m[i][b] = x;
-                        l[i][b] *= f;
-#pragma unroll
-                        for (int d = 0; d < 8; ++d) {
-                            o[i][d][2 * b] *= f;
-                            o[i][d][2 * b + 1] *= f;
-                        }
-                    }
-            }
-            // P as A fragments of two 16-key steps.
-            uint32_t ph[MT][2][4], pl[MT][2][P2 ? 4 : 1];
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int n = 0; n < 4; ++n)
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const float e0 = score_exp2(s[i][n][2 * b] - m[i][b]), e1 = score_exp2(s[i][n][2 * b + 1] - m[i][b]);
-                        l[i][b] += e0 + e1;
-                        const uint32_t w = pack_bf16x2(e0, e1);
-                        ph[i][n >> 1][2 * (n & 1) + b] = w;
-                        if constexpr (P2) pl[i][n >> 1][2 * (n & 1) + b] = pack_bf16x2(e0 - bf16lo(w), e1 - bf16hi(w));
-                    }
-            // O += P V: dims 8 d + 2 t (+1) in o[i][d].
-            bool bad = false;
-#pragma unroll
-            for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-                for (int d2 = 0; d2 < 4; ++d2) {
-                    uint32_t vb[4];
-                    const int key = 16 * kk + v_row;
-                    ldsm_x4_t(va + key * 128 + (((2 * d2 + v_chunk) ^ (key & 7)) << 4), vb);
-                    if (edge) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) bad |= drop_not_finite(vb[e]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        mma_bf16(o[i][2 * d2], ph[i][kk], vb[0], vb[1]);
-                        mma_bf16(o[i][2 * d2 + 1], ph[i][kk], vb[2], vb[3]);
-                        if constexpr (P2) {
-                            mma_bf16(o[i][2 * d2], pl[i][kk], vb[0], vb[1]);
-                            mma_bf16(o[i][2 * d2 + 1], pl[i][kk], vb[2], vb[3]);
+                        for (int y = 0; y < 2; ++y) {
+                            const bool sees = x < keys && x >= row_lo[y] && x <= row_hi[y] && (node < 0 || (row_line[y] >> (node & 63) & 1));
+                            const uint32_t rows = __ballot_sync(0xffffffffu, sees);
+                            if (lane == k) seen[y] = rows;
                         }
                     }
                 }
-            if (edge && __any_sync(0xffffffffu, bad)) {
-                for (int key = 0; key < hd.n; ++key) {
+                float at = (float)slot;  // the key's position
+                if (biased && slot >= base_slot) at = R->pos[min(slot - base_slot, NR - 1)];
+                ok = ok && __all_sync(0xffffffffu, mbar_wait(&b->sfull, i & 1));
+                float s[NR];
+                float past = -INFINITY;  // how far the scores pass their rows' maxima
+                if (ok) {
+                    fa_after();
 #pragma unroll
-                    for (int i = 0; i < MT; ++i)
+                    for (int g = 0; g < 4; ++g)
+                        if (g < groups) ld16(lanes + 16 * g, s + 16 * g);
+                    fa_wait_ld();
+                    fa_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&b->sfree);
 #pragma unroll
-                        for (int b = 0; b < 2; ++b) {
-                            const int r = rbase + 16 * i + g + 8 * b;
-                            if (r >= hd.nrows || !sees_of(a.rows, hd.row0 + r)(hd.slot + key)) continue;
+                    for (int g = 0; g < 4; ++g) {
+                        if (g >= groups) continue;
+                        float* x = s + 16 * g;
+                        if (CAP == kCapFast) cap_fast<16>(x, a.rule.cap);
+                        if (CAP == kCapExact) {
 #pragma unroll
-                            for (int d = 0; d < 8; ++d) {  // dims 8 d + 2 t, + 1: chunk d, bytes 4 t
-                                const uint32_t w = *reinterpret_cast<const uint32_t*>(
-                                    kt + S::kStageBytes / 2 + key * 128 + ((d ^ (key & 7)) << 4) + 4 * t);
-                                if (!isfinite(bf16lo(w))) o[i][d][2 * b] += bf16lo(w);
-                                if (!isfinite(bf16hi(w))) o[i][d][2 * b + 1] += bf16hi(w);
+                            for (int j = 0; j < 16; ++j) x[j] = cap_exact(x[j], a.rule.cap);
+                        }
+                        if (biased) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) x[j] = fmaf(-slope, fabsf(R->pos[16 * g + j] - at), x[j]);
+                        }
+                        if (!whole) {
+                            const uint32_t bits = seen[g >> 1] >> (16 * (g & 1));
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) x[j] = bits >> j & 1 ? x[j] : -INFINITY;
+                        }
+                        // From here on the scores are past their rows' maxima (or BOUNDED's references, 0 without a bias).
+                        if (!BOUNDED || biased) {
+#pragma unroll
+                            for (int j = 0; j < 16; j += 4) {
+                                const float4 m = *reinterpret_cast<const float4*>(&R->m[16 * g + j]);
+                                x[j] -= m.x, x[j + 1] -= m.y, x[j + 2] -= m.z, x[j + 3] -= m.w;
                             }
                         }
+                        if (!BOUNDED) {
+#pragma unroll
+                            for (int j = 0; j < 16; j += 2) past = fa_max3(past, x[j], x[j + 1]);
+                        }
+                    }
                 }
+                if (!BOUNDED && (head_any(hl, !ok || past > kRaiseR) || fresh)) {
+                    // The item's most past each row's maximum: 32 rows over a warp's keys by halving, each lane
+                    // left with one row, then over the warps. It becomes the maximum of rows that have none, and raises
+                    // rows that it passes by more than kRaiseR.
+                    if (key < NR) R->top[key] = ordered(kScoreLow);
+                    if (head_any(hl, !ok)) break;
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        if (2 * y >= groups) continue;
+                        float v[16];
+                        const bool up = lane & 16;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const bool both = 2 * y + 1 < groups;  // a half group of rows that are not there: lowest
+                            const float lo = s[32 * y + j], hi = both ? s[32 * y + 16 + j] : kScoreLow;
+                            v[j] = fmaxf(up ? hi : lo, __shfl_xor_sync(0xffffffffu, up ? lo : hi, 16));
+                        }
+#pragma unroll
+                        for (int d = 8; d > 0; d >>= 1) {
+                            const bool u = lane & d;
+#pragma unroll
+                            for (int j = 0; j < d; ++j) {
+                                const float lo = v[j], hi = v[j + d];
+                                v[j] = fmaxf(u ? hi : lo, __shfl_xor_sync(0xffffffffu, u ? lo : hi, d));
+                            }
+                        }
+                        atomicMax(&R->top[32 * y + lane], ordered(v[0]));
+                    }
+                    head_any(hl, false);
+                    if (key < NR) {
+                        const float x = unordered(R->top[key]);
+                        const bool first = !R->has[key] && x > kScoreLow, raise = R->has[key] && x > kRaiseR;
+                        R->shift[key] = first || raise ? x : 0.f;
+                        R->scale[key] = raise ? score_exp2(-x) : 1.f;
+                        if (first || raise) R->m[key] += x;
+                        if (first) R->has[key] = 1;
+                    }
+                    if (fresh) fresh = head_any(hl, key < w.nrows && key < NR && !R->has[key & (NR - 1)]);
+                    if (it > 0) ok = __all_sync(0xffffffffu, mbar_wait(&b->odone, (i - 1) & 1));
+                    if (head_any(hl, !ok)) break;
+                    if (it > 0) {  // O of the piece's items before this one
+                        fa_after();
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            if (g >= groups) continue;
+                            float o[16];
+                            uint32_t x[16];
+                            ld16(lanes + 64 + 16 * g, o);
+                            fa_wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(o[j] * R->scale[16 * g + j]);
+                            st16(lanes + 64 + 16 * g, x);
+                        }
+                        wait_st();
+                    }
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        if (g >= groups) continue;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) s[16 * g + j] -= R->shift[16 * g + j];
+                    }
+                } else if (i > 0) {  // P V of the item before has read P
+                    ok = ok && __all_sync(0xffffffffu, mbar_wait(&b->odone, (i - 1) & 1));
+                }
+                if (ok) {
+                    fa_after();
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        if (g >= groups) continue;
+                        uint32_t hi[8], lo[P2 ? 8 : 1];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float e0 = score_exp2(s[16 * g + 2 * j]), e1 = score_exp2(s[16 * g + 2 * j + 1]);
+                            hi[j] = pack_bf16x2(e0, e1);
+                            if constexpr (P2) lo[j] = pack_bf16x2(e0 - bf16lo(hi[j]), e1 - bf16hi(hi[j]));
+                        }
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const int chunk = (2 * g + q) ^ (key & 7);
+                            *reinterpret_cast<uint4*>(pt + 16 * chunk) = make_uint4(hi[4 * q], hi[4 * q + 1], hi[4 * q + 2], hi[4 * q + 3]);
+                            if constexpr (P2)
+                                *reinterpret_cast<uint4*>(pt + kTile + 16 * chunk) = make_uint4(lo[4 * q], lo[4 * q + 1], lo[4 * q + 2], lo[4 * q + 3]);
+                        }
+                    }
+                    if (!whole) {
+                        ok = __all_sync(0xffffffffu, mbar_wait(&b->vfull[i % kSlots], (i / kSlots) & 1));
+                        if (ok) clean_v(sm + L::kV + (hl * kSlots + i % kSlots) * kTile, key, (seen[0] | seen[1]) == 0, &R->bad);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // P, and V where it was cleaned
+                    fa_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&b->pfull);
+                }
+            }
+            // The piece's end: O^T has a dim a lane (threads 0-63), the rows' sums in lane 64.
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(&b->odone, (i - 1) & 1));
+            float o[NR];
+            if (ok && (warp & 3) < 3) {
+                fa_after();
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    if (g < groups) ld16(lanes + 64 + 16 * g, o + 16 * g);
+                fa_wait_ld();
+                fa_before();  // O is read before the next piece's first P V (through pfull)
+                if (key == NR) {
+#pragma unroll
+                    for (int r = 0; r < NR; ++r)
+                        if (r < 16 * groups) R->sum[r] = !w.whole ? o[r] : o[r] == 0.f ? 0.f : 1.f / o[r];  // zeros for a row that sees nothing
+                }
+            }
+            if (head_any(hl, !ok)) {
+                ok = false;
+                break;
+            }
+            if (key < NR) {
+                if (R->bad) add_not_finite<NR>(a, *R, w, base_slot, head, key, o);
+                const long long at = (long long)w.row0 * a.ld + head * kHeadDim + key;
+                // Record 2 c of a piece that began before this CTA's range, 2 c + 1 of one that begins in it.
+                float* rec = a.part + ((long long)(2 * c + (w.begins ? 1 : 0)) * a.heads + head) * NR * kPartStride;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    if (g >= groups) continue;
+                    if (w.whole) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const int r = 16 * g + j;
+                            const float y = o[r] * R->sum[r];
+                            if (r < w.nrows) {
+                                if constexpr (P2) static_cast<float*>(a.out)[at + (long long)r * a.ld] = y;
+                                else static_cast<__nv_bfloat16*>(a.out)[at + (long long)r * a.ld] = __float2bfloat16_rn(y);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (16 * g + j < w.nrows) rec[(16 * g + j) * kPartStride + key] = o[16 * g + j];
+                    }
+                }
+                if (!w.whole && key < w.nrows)
+                    *reinterpret_cast<float2*>(rec + key * kPartStride + NR) = make_float2(BOUNDED || R->has[key] ? R->m[key] : kScoreLow, R->sum[key]);
+            }
+            head_any(hl, false);  // the rows' arrays are the next block's from here
+        }
+        if (!ok && lane == 0) set_error(a.err, DEV_ERR_TIMEOUT);
+    } else {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
+      if ((warp == 8 || warp == 8 + HC - 1) && lane == 0 && !idle) {
+        // ---- MMA issuer of a head -------------------------------------------------------------------
+        const int hl = warp - 8;
+        HeadBars* b = bars_of(hl);
+        const uint32_t ts = tmem + 128 * hl, to = ts + 64;
+        const uint32_t q = base + L::kQ + hl * 2 * kQTile, k = base + L::kK + hl * kSlots * kTile,
+                       v = base + L::kV + hl * kSlots * kTile, p = base + L::kP + hl * (P2 ? 2 : 1) * kTile;
+        auto k_full = [&](int i) { return &b->kfull[i % kSlots]; };
+        auto issue_s = [&](int i, uint32_t rows, bool last) {
+            fa_after();
+            const uint64_t dk = desc_k(k + (i % kSlots) * kTile), qh = desc_k(q), ql = desc_k(q + kQTile);
+            const uint32_t idesc = kIdescBase | rows / 8 << 17;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {  // 64 dims, 16 (32 bytes) a step
+                fa_mma_ss(ts, dk + 2 * d, qh + 2 * d, idesc, d ? 1u : 0u);
+                fa_mma_ss(ts, dk + 2 * d, ql + 2 * d, idesc, 1u);
+            }
+            fa_commit(&b->sfull);
+            fa_commit(&b->kempty[i % kSlots]);
+            if (last) fa_commit(&b->qfree);
+        };
+        auto issue_pv = [&](int i, uint32_t rows, bool first) {
+            fa_after();
+            const uint32_t vt = v + (i % kSlots) * kTile;
+            // A: dims 0-63 of V, then the ones tile, 128-byte rows of keys (both operands MN-major).
+            const uint64_t dv = (uint64_t)((vt >> 4) & 0x3FFFu) | ((uint64_t)((base + L::kOnes - vt) >> 4) << 16) |
+                                ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
+            const uint64_t dp = desc_mn(p);
+            const uint32_t idesc = kIdescBase | rows / 8 << 17 | 1u << 15 | 1u << 16;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {  // 128 keys, 16 (2048 bytes) a step
+                fa_mma_ss(to, dv + 128 * d, dp + 128 * d, idesc, !first || d ? 1u : 0u);
+                if (P2) fa_mma_ss(to, dv + 128 * d, dp + (kTile >> 4) + 128 * d, idesc, 1u);
+            }
+            fa_commit(&b->odone);
+            fa_commit(&b->vempty[i % kSlots]);
+        };
+        bool ok = true;
+        int i = 0, piece = 0;
+        uint32_t last_rows = 0;   // of the item before, whose P V is still to come
+        bool last_first = false;
+        auto pv_before = [&]() {
+            ok = ok && mbar_wait(&b->pfull, (i - 1) & 1) && mbar_wait(&b->vfull[(i - 1) % kSlots], ((i - 1) / kSlots) & 1);
+            if (ok) issue_pv(i - 1, last_rows, last_first);
+        };
+        Walk w(a, c, total, G);
+        for (; ok && w.next(); ++piece) {
+            const int n = w.items();
+            const uint32_t rows = (uint32_t)((w.nrows + 15) / 16 * 16);
+            for (int it = 0; it < n && ok; ++it, ++i) {
+                // S goes first where its keys are there; else P V of the item before, then S.
+                const bool there = i == 0 || (it > 0 && mbar_test_wait(k_full(i), (i / kSlots) & 1));
+                if (!there) pv_before();
+                ok = ok && mbar_wait(k_full(i), (i / kSlots) & 1) && mbar_wait(&b->qready, piece & 1) &&
+                     (i == 0 || mbar_wait(&b->sfree, (i - 1) & 1));
+                if (ok) issue_s(i, rows, it == n - 1);
+                if (there && i > 0) pv_before();
+                last_rows = rows;
+                last_first = it == 0;
             }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[st]);
-        if (!(hd.flags & kRLast) || !any) continue;
-        // The end of this CTA's piece of the block.
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                float x = l[i][b];
-                x += __shfl_xor_sync(0xffffffffu, x, 1);
-                x += __shfl_xor_sync(0xffffffffu, x, 2);
-                const int r = rbase + 16 * i + g + 8 * b;
-                if (r >= hd.nrows) continue;
-                if (hd.flags & kRWhole) {
-                    const float inv = x == 0.f ? 0.f : 1.f / x;  // a row that sees nothing: zeros
-                    const long long at = (long long)(hd.row0 + r) * a.ld + head * kHeadDim + 2 * t;
-#pragma unroll
-                    for (int d = 0; d < 8; ++d) {
-                        const float y0 = o[i][d][2 * b] * inv, y1 = o[i][d][2 * b + 1] * inv;
-                        if constexpr (P2) *reinterpret_cast<float2*>(static_cast<float*>(a.out) + at + 8 * d) = make_float2(y0, y1);
-                        else *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + at + 8 * d) = pack_bf16x2(y0, y1);
-                    }
-                } else {
-                    // Record 2 c of a piece that began before this CTA's range, 2 c + 1 of one that begins in it.
-                    float* rec = a.part + (((long long)(2 * c + (hd.flags & kRBegins ? 1 : 0)) * a.heads + head) * S::kRows + r) * kPartStride;
-#pragma unroll
-                    for (int d = 0; d < 8; ++d)
-                        *reinterpret_cast<float2*>(rec + 8 * d + 2 * t) = make_float2(o[i][d][2 * b], o[i][d][2 * b + 1]);
-                    if (t == 0) *reinterpret_cast<float2*>(rec + 64) = make_float2(m[i][b], x);
-                }
+        if (i > 0) pv_before();
+        if (!ok) set_error(a.err, DEV_ERR_TIMEOUT);
+      } else if (warp == 10 && lane == 0 && !idle) {
+        // ---- producer -------------------------------------------------------------------------------
+        bool ok = true;
+        int i = 0, piece = 0, q_out = 0, k_out = 0, v_out = 0;  // copies are issued for all heads up to these
+        Walk w(a, c, total, G);
+        for (; ok && w.next(); ++piece) {
+            const int sid = max(a.rows.stream[w.row0], 0);  // a refused tree reads slot 0 and sees nothing
+            for (int hl = 0; hl < HC && ok; ++hl) {
+                HeadBars* b = bars_of(hl);
+                if (piece > 0 && !(ok = mbar_wait(&b->qfree, (piece - 1) & 1))) break;
+                const uint32_t q = base + L::kQ + hl * 2 * kQTile;
+                mbar_arrive_expect_tx(&b->qready, 2 * kQTile);
+                fa_tma(q, &tm_qh, (head0 + hl) * kHeadDim, w.row0, &b->qready);
+                fa_tma(q + kQTile, &tm_ql, (head0 + hl) * kHeadDim, w.row0, &b->qready);
+                q_out = piece * HC + hl + 1;
             }
+            const int n = w.items();
+            for (int it = 0; it < n && ok; ++it, ++i) {
+                const int slot = i % kSlots;
+                const uint32_t ph = ((i / kSlots) & 1) ^ 1;
+                for (int kv = 0; kv < 2 && ok; ++kv)
+                    for (int hl = 0; hl < HC && ok; ++hl) {
+                        HeadBars* b = bars_of(hl);
+                        const int head = head0 + hl;
+                        const int y = (int)(((long long)(head / kGroupHeads) * a.num_streams + sid) * a.capacity) + w.lo + w.s0 + it * KT;
+                        if (i >= kSlots && !(ok = mbar_wait(kv ? &b->vempty[slot] : &b->kempty[slot], ph))) break;
+                        uint64_t* full = kv ? &b->vfull[slot] : &b->kfull[slot];
+                        mbar_arrive_expect_tx(full, kTile);
+                        fa_tma(base + (kv ? L::kV : L::kK) + (hl * kSlots + slot) * kTile, kv ? &tm_v : &tm_k,
+                               head % kGroupHeads * kHeadDim, y, full);
+                        (kv ? v_out : k_out) = i * HC + hl + 1;
+                    }
+            }
+        }
+        if (!ok) set_error(a.err, DEV_ERR_TIMEOUT);
+        // The last copies into each buffer land before the shared memory goes (a completed phase returns at
+        // once). Copy j of a kind is head j % HC's item (or piece) j / HC.
+        for (int j = max(0, q_out - HC); j < q_out; ++j) mbar_wait(&bars_of(j % HC)->qready, (j / HC) & 1);
+        for (int j = max(0, k_out - HC * kSlots); j < k_out; ++j)
+            mbar_wait(&bars_of(j % HC)->kfull[j / HC % kSlots], (j / HC / kSlots) & 1);
+        for (int j = max(0, v_out - HC * kSlots); j < v_out; ++j)
+            mbar_wait(&bars_of(j % HC)->vfull[j / HC % kSlots], (j / HC / kSlots) & 1);
+      }
+    }
+    fa_before();
+    __syncthreads();
+    if (warp == 0) {
+        fa_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
     }
 }
 
@@ -475,50 +606,51 @@ __global__ void __launch_bounds__(256) score_rows_merge_kernel(ScoreRowsArgs a, 
     else *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + at) = pack_bf16x2(x0 * inv, x1 * inv);
 }
 
-template <class S, int CAP, bool P2>
-void launch_shape(const ScoreRowsArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int grid, cudaStream_t s) {
-    set_max_dynamic_smem(reinterpret_cast<const void*>(score_rows_kernel<S, CAP, P2>), S::kSmem);
-    launch_k(score_rows_kernel<S, CAP, P2>, dim3(grid, a.heads / S::kHeads), dim3(kThreadsR), S::kSmem, s, a, mk, mv);
-    if (grid > 1) launch_k(score_rows_merge_kernel<P2>, dim3(a.n_units, a.heads, S::kRows / 8), dim3(256), 0, s, a, grid, S::kRows);
+template <bool P2>
+void merge(const ScoreRowsArgs& a, int grid, cudaStream_t s) {
+    if (grid > 1)
+        launch_k(score_rows_merge_kernel<P2>, dim3(a.n_units, a.heads, (a.most_rows + 7) / 8), dim3(256), 0, s, a, grid, NR);
 }
 
-template <class S>
-void launch_rules(const ScoreRowsArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int grid, cudaStream_t s) {
-    const int cap = score_cap_mode(a.rule.cap, !a.out_bf16);
-    if (a.out_bf16) {
-        if (cap == kCapNone) launch_shape<S, kCapNone, false>(a, mk, mv, grid, s);
-        else if (cap == kCapFast) launch_shape<S, kCapFast, false>(a, mk, mv, grid, s);
-        else launch_shape<S, kCapExact, false>(a, mk, mv, grid, s);
-    } else {
-        if (cap == kCapNone) launch_shape<S, kCapNone, true>(a, mk, mv, grid, s);
-        else launch_shape<S, kCapExact, true>(a, mk, mv, grid, s);
-    }
+template <int HC, int CAP, bool BOUNDED, bool P2>
+void launch_rules(const ScoreRowsArgs& a, const CUtensorMap* m, int grid, cudaStream_t s) {
+    auto kernel = score_rows_kernel<HC, CAP, BOUNDED, P2>;
+    constexpr int smem = Smem<HC, P2 ? 2 : 1>::kBytes;
+    static_assert(smem <= 227 * 1024, "a CTA per SM");
+    set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+    launch_k(kernel, dim3(grid, a.heads / HC), dim3(kThreadsR), smem, s, a, m[0], m[1], m[2], m[3]);
+    merge<P2>(a, grid, s);
 }
-
-using Rows16 = Shape<1, 1>;
-using Rows32 = Shape<2, 1>;
-using Rows64 = Shape<2, 2>;
 
 }  // namespace
 
-int score_rows_block(int most_rows) { return most_rows <= Rows16::kRows ? Rows16::kRows : most_rows <= Rows32::kRows ? Rows32::kRows : Rows64::kRows; }
-
-int score_rows_grid(int block, int heads, int sms) {
-    const int slabs = heads / (block == Rows64::kRows ? Rows64::kHeads : Rows16::kHeads);
+int score_rows_grid(bool out_bf16, int heads, int sms) {
+    const int slabs = heads / (out_bf16 ? 2 : 1);
     return sms / slabs > 1 ? sms / slabs : 1;
 }
 
-size_t score_rows_part_floats(int block, int heads, int grid) { return (size_t)2 * grid * heads * block * kPartStride; }
+size_t score_rows_part_floats(int heads, int grid) { return (size_t)2 * grid * heads * NR * kPartStride; }
 
-bool launch_score_rows(const ScoreRowsArgs& a, int block, int grid, cudaStream_t s) {
-    CUtensorMap mk, mv;
-    const int heads = block == Rows64::kRows ? Rows64::kHeads : Rows16::kHeads;
+bool launch_score_rows(const ScoreRowsArgs& a, int grid, cudaStream_t s) {
+    CUtensorMap m[4];
     const long long rows = (long long)(a.heads / kGroupHeads) * a.num_streams * a.capacity;
-    if (rows >= (1LL << 31) || !bf16_heads_map(&mk, a.k_cache, rows, KC, heads) || !bf16_heads_map(&mv, a.v_cache, rows, KC, heads))
+    if (rows >= (1LL << 31) || !bf16_rows_map(&m[0], a.k_cache, rows, kRowWidth, kHeadDim, KT) ||
+        !bf16_rows_map(&m[1], a.v_cache, rows, kRowWidth, kHeadDim, KT) ||
+        !bf16_rows_map(&m[2], a.q_hi, a.n_rows, a.ld, kHeadDim, NR) || !bf16_rows_map(&m[3], a.q_lo, a.n_rows, a.ld, kHeadDim, NR))
         return false;
-    if (block == Rows16::kRows) launch_rules<Rows16>(a, mk, mv, grid, s);
-    else if (block == Rows32::kRows) launch_rules<Rows32>(a, mk, mv, grid, s);
-    else launch_rules<Rows64>(a, mk, mv, grid, s);
+    const int cap = score_cap_mode(a.rule.cap, !a.out_bf16);
+    if (!a.out_bf16) {
+        if (cap == kCapNone) launch_rules<1, kCapNone, false, true>(a, m, grid, s);
+        else launch_rules<1, kCapExact, false, true>(a, m, grid, s);
+    } else if (cap == kCapNone) {
+        launch_rules<2, kCapNone, false, false>(a, m, grid, s);
+    } else if (cap == kCapExact) {
+        launch_rules<2, kCapExact, false, false>(a, m, grid, s);
+    } else if (a.rule.cap <= kScoreBoundedCap) {
+        launch_rules<2, kCapFast, true, false>(a, m, grid, s);
+    } else {
+        launch_rules<2, kCapFast, false, false>(a, m, grid, s);
+    }
     return true;
 }
 

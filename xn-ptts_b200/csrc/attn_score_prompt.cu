@@ -48,7 +48,6 @@ constexpr uint32_t kCols = 256, kColS = 0, kColO = 128, kColP = 192;
 constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((KT / 8) << 17) | (8u << 24);
 constexpr uint32_t kIdescPV = (1u << 4) | (1u << 7) | (1u << 10) | (8u << 17) | (8u << 24) | (1u << 16);
 constexpr float kRaiseP = 8.f;
-constexpr float kBoundedCap = 40.f;  // 40 log2(e) < 58: weights and sums of 2^58 stay far inside f32 and bf16
 
 // Single buffers for S, P and O: item i completes phase i of sfull, sfree, pfull and odone, head hh
 // phase hh of qready and qfree, and each waiter asks for every phase (or for one that its last wait on
@@ -57,26 +56,6 @@ struct Bars {
     uint64_t qready, kfull[kSlots], kempty[kSlots], vfull[kSlots], vempty[kSlots], qfree, sfull, sfree, pfull, odone;
 };
 
-__device__ __forceinline__ void st16(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
-__device__ __forceinline__ void ld16(uint32_t taddr, float* r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
-          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
-        : "r"(taddr));
-}
-__device__ __forceinline__ void ld8(uint32_t taddr, float* r) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7])
-                 : "r"(taddr));
-}
-__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // The values of slots lo .. hi that are not finite, from the cache, onto 32 dims of a row.
 __device__ __forceinline__ void add_not_finite(const ScorePromptArgs& a, int kv_row, int x, int lo, int hi, float* o) {
@@ -89,36 +68,6 @@ __device__ __forceinline__ void add_not_finite(const ScorePromptArgs& a, int kv_
         }
 }
 
-// Key `key` of a V tile: zeros if the key is gone, else without what is not finite
-// (x 0 is NaN then), which `bad` records. Swizzled 16-byte chunks; visible to the products afterwards.
-__device__ __forceinline__ void clean_v(unsigned char* tile, int key, bool gone, int* bad) {
-    uint4* v = reinterpret_cast<uint4*>(tile + key * 128);
-    const uint32_t zero = 0;
-    uint32_t probe = 0;
-    uint4 w[8];
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-        w[c] = v[c ^ (key & 7)];
-        const uint32_t* u = &w[c].x;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(probe) : "r"(u[j]), "r"(zero));
-    }
-    const bool drop = (probe & 0x7fff7fffu) != 0;  // NaN in either half
-    if (gone || drop) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            uint32_t* u = &w[c].x;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (gone) u[j] = 0u;
-                else drop_not_finite(u[j]);
-            }
-            v[c ^ (key & 7)] = w[c];
-        }
-        if (!gone) *bad = 1;
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
 // 32 scores of a row: capped, biased (`ahead` = position - first key), -inf outside keys from .. to
 // (unless `whole`: every key is visible).
 template <int CAP, bool BIAS>
@@ -511,7 +460,7 @@ bool launch_score_prompt(const ScorePromptArgs& a, cudaStream_t s) {
         launch_bias<kCapNone, false, false>(a, m, s);
     } else if (cap == kCapExact) {
         launch_bias<kCapExact, false, false>(a, m, s);
-    } else if (a.rule.cap <= kBoundedCap) {
+    } else if (a.rule.cap <= kScoreBoundedCap) {
         launch_bias<kCapFast, true, false>(a, m, s);
     } else {
         launch_bias<kCapFast, false, false>(a, m, s);

@@ -284,9 +284,6 @@ bool launch_prefill_attn_fa(const PrefillArgs& a, const int2* tiles, int n_tiles
 // 128-byte swizzle (linear_tc.cu).
 bool bf16_rows_map(CUtensorMap* out, const void* ptr, long long rows, int cols, int box_cols, int box_rows,
                    int ld = 0);
-// Tensor map of bf16 cache rows [rows][8 heads][64] as (dim, row, head), box 64 x box_rows x
-// box_heads: shared memory gets [head][row][64], 128-byte swizzle (linear_tc.cu).
-bool bf16_heads_map(CUtensorMap* out, const void* ptr, long long rows, int box_rows, int box_heads);
 
 // ---- int8 linear (linear.cu) ----------------------------------------------------------
 

@@ -1524,18 +1524,6 @@ bool bf16_rows_map(CUtensorMap* out, const void* ptr, long long rows, int cols, 
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool bf16_heads_map(CUtensorMap* out, const void* ptr, long long rows, int box_rows, int box_heads) {
-    EncodeTiled enc = encoder();
-    if (!enc || rows <= 0) return false;
-    const cuuint64_t dims[3] = {(cuuint64_t)kHeadDim, (cuuint64_t)rows, (cuuint64_t)kGroupHeads};
-    const cuuint64_t strides[2] = {(cuuint64_t)kRowWidth * 2, (cuuint64_t)kHeadDim * 2};
-    const cuuint32_t box[3] = {(cuuint32_t)kHeadDim, (cuuint32_t)box_rows, (cuuint32_t)box_heads};
-    const cuuint32_t elem[3] = {1, 1, 1};
-    return enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, elem,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 bool linear_tc_supported(const LinearArgs& a) {
     return (a.wh != nullptr || a.w != nullptr) && a.M > 0 && a.N % FT == 0 && a.K % 8 == 0 && a.splits >= 1 &&
            a.K % a.splits == 0 && (a.K / a.splits) % KS == 0;

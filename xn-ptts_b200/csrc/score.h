@@ -87,6 +87,8 @@ void launch_score_core(const ScoreCoreArgs& a, bool cache_bf16, cudaStream_t s);
 // without a cap).
 enum { kCapNone = 0, kCapFast = 1, kCapExact = 2 };
 constexpr float kScoreFastCap = 128.f;
+// Caps this small bound the scores: 40 log2(e) < 58, and weights and sums of 2^58 stay far inside f32 and bf16.
+constexpr float kScoreBoundedCap = 40.f;
 inline int score_cap_mode(float cap, bool out_f32) {
     return cap == 0.f ? kCapNone : (!out_f32 && cap <= kScoreFastCap ? kCapFast : kCapExact);
 }
@@ -95,9 +97,8 @@ inline float score_q_scale(float cap, bool out_f32) {
     return score_cap_mode(cap, out_f32) == kCapFast ? 0.125f / cap : 0.125f * log2e;
 }
 
-// Few rows over a whole cache on mma.sync, bf16 caches (attn_rows.cu): blocks of up to
-// score_rows_block(most rows of a sequence) rows, the plan's units. False: the tensor maps could
-// not be made, nothing launched.
+// Few rows over a whole cache, bf16 caches (attn_rows.cu): blocks of up to kTreeNodes rows of one
+// sequence, the plan's units. False: the tensor maps could not be made, nothing launched.
 struct ScoreRowsArgs {
     const void* k_cache;  // the layer
     const void* v_cache;
@@ -105,7 +106,7 @@ struct ScoreRowsArgs {
     const __nv_bfloat16* q_lo;
     void* out;            // [n_rows][ld]
     bool out_bf16;
-    int ld, heads, num_streams, capacity;
+    int ld, heads, num_streams, capacity, n_rows;
     ScoreRows rows;
     ScoreRule rule;
     const int2* blocks;   // [n_units]
@@ -113,13 +114,13 @@ struct ScoreRowsArgs {
     const int32_t* prefix;
     const int32_t* unit_lo;
     const int32_t* cta_first;
+    int most_rows;        // of a block
     float* part;          // score_rows_part_floats
     uint32_t* err;
 };
-int score_rows_block(int most_rows);
-int score_rows_grid(int block, int heads, int sms);  // CTAs along the keys (the plan's grid)
-size_t score_rows_part_floats(int block, int heads, int grid);
-bool launch_score_rows(const ScoreRowsArgs& a, int block, int grid, cudaStream_t s);
+int score_rows_grid(bool out_bf16, int heads, int sms);  // CTAs along the keys (the plan's grid)
+size_t score_rows_part_floats(int heads, int grid);
+bool launch_score_rows(const ScoreRowsArgs& a, int grid, cudaStream_t s);
 
 // Prompts on tcgen05, bf16 caches (attn_score_prompt.cu): tiles (first row, rows) of up to 128 rows
 // of one sequence. False: the tensor maps could not be made, nothing launched.
