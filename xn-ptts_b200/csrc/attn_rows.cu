@@ -122,19 +122,22 @@ struct Walk {
     __device__ int items() const { return (s1 - s0 + KT - 1) / KT; }
 };
 
-// The values of the piece's keys that are not finite, from the cache, for one dim of the rows that see them.
-template <int N>
+// The values of the piece's keys that are not finite, from the cache, for one dim of the rows that see them
+// (rows r0 .. r0 + 15).
 __device__ __forceinline__ void add_not_finite(const ScoreRowsArgs& a, const HeadRows& R, const Walk& w, int base_slot,
-                                               int head, int dim, float* o) {
+                                               int head, int dim, int r0, float* o) {
     const int sid = max(a.rows.stream[w.row0], 0);
     const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.v_cache) + kv_offset(sid, w.lo, head, a.num_streams, a.capacity) + dim;
+#pragma unroll 1
     for (int j = w.s0; j < w.s1; ++j) {
         const float x = __bfloat162float(v[(long long)j * kRowWidth]);
         if (isfinite(x)) continue;
         const int slot = w.lo + j, node = slot - base_slot;
 #pragma unroll
-        for (int r = 0; r < N; ++r)
-            if (r < w.nrows && slot >= R.lo[r] && slot <= R.hi[r] && (node < 0 || (R.lineage[r] >> node & 1))) o[r] += x;
+        for (int i = 0; i < 16; ++i) {
+            const int r = r0 + i;
+            if (r < w.nrows && slot >= R.lo[r] && slot <= R.hi[r] && (node < 0 || (R.lineage[r] >> node & 1))) o[i] += x;
+        }
     }
 }
 
@@ -239,17 +242,28 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
                 const int slot0 = w.lo + w.s0 + it * KT, slot = slot0 + key;
                 const int count = min(KT, w.s1 - w.s0 - it * KT);  // keys of this item in this CTA's range
                 const bool whole = count == KT && slot0 >= full_lo && slot0 + KT - 1 <= full_hi;
-                // Rows that see this thread's key: key by key, the lanes say it for their two rows.
+                // Rows that see this thread's key, a bit each: every lane has its two rows' 32 keys of the
+                // warp, and 32 ballots turn rows of keys into keys of rows.
                 uint32_t seen[2] = {~0u, ~0u};
                 if (!whole) {
-                    const int mine = slot0 + 32 * (warp & 3), keys = w.lo + w.s1;  // this warp's keys; the range's end
-#pragma unroll 4
-                    for (int k = 0; k < 32; ++k) {
-                        const int x = mine + k, node = x - base_slot;
+                    const int mine = slot0 + 32 * (warp & 3), last = w.lo + w.s1 - 1;  // the warp's first key; the range's last
+                    const int past_base = mine - base_slot;                           // the first key's node, if not negative
 #pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            const bool sees = x < keys && x >= row_lo[y] && x <= row_hi[y] && (node < 0 || (row_line[y] >> (node & 63) & 1));
-                            const uint32_t rows = __ballot_sync(0xffffffffu, sees);
+                    for (int y = 0; y < 2; ++y) {
+                        if (32 * y >= w.nrows) {
+                            seen[y] = 0;
+                            continue;
+                        }
+                        const int from = row_lo[y] - mine, to = min(row_hi[y], last) - mine;
+                        uint32_t keys = (from <= 0 ? ~0u : from > 31 ? 0u : ~0u << from) & (to >= 31 ? ~0u : to < 0 ? 0u : ~0u >> (31 - to));
+                        if (past_base > -32) {  // cached keys, then nodes in the row's lineage
+                            const unsigned long long line = past_base >= 0 ? (past_base < NR ? row_line[y] >> past_base : 0ull)
+                                                                           : row_line[y] << -past_base | ((1ull << -past_base) - 1);
+                            keys &= (uint32_t)line;
+                        }
+#pragma unroll 8
+                        for (int k = 0; k < 32; ++k) {
+                            const uint32_t rows = __ballot_sync(0xffffffffu, keys >> k & 1);
                             if (lane == k) seen[y] = rows;
                         }
                     }
@@ -396,50 +410,53 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
             }
             // The piece's end: O^T has a dim a lane (threads 0-63), the rows' sums in lane 64.
             ok = ok && __all_sync(0xffffffffu, mbar_wait(&b->odone, (i - 1) & 1));
-            float o[NR];
-            if (ok && (warp & 3) < 3) {
+            if (ok && (warp & 3) == 2) {
                 fa_after();
+#pragma unroll 1
+                for (int g = 0; g < groups; ++g) {
+                    float o[16];
+                    ld16(lanes + 64 + 16 * g, o);
+                    fa_wait_ld();
+                    if (lane == 0) {
 #pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    if (g < groups) ld16(lanes + 64 + 16 * g, o + 16 * g);
-                fa_wait_ld();
-                fa_before();  // O is read before the next piece's first P V (through pfull)
-                if (key == NR) {
-#pragma unroll
-                    for (int r = 0; r < NR; ++r)
-                        if (r < 16 * groups) R->sum[r] = !w.whole ? o[r] : o[r] == 0.f ? 0.f : 1.f / o[r];  // zeros for a row that sees nothing
+                        for (int j = 0; j < 16; j += 4)
+                            *reinterpret_cast<float4*>(&R->sum[16 * g + j]) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                    }
                 }
+                __syncwarp();
+                // As factors of a finished block's rows: zeros for those that see nothing.
+                for (int r = lane; w.whole && r < NR; r += 32) R->sum[r] = R->sum[r] == 0.f ? 0.f : 1.f / R->sum[r];
             }
             if (head_any(hl, !ok)) {
                 ok = false;
                 break;
             }
             if (key < NR) {
-                if (R->bad) add_not_finite<NR>(a, *R, w, base_slot, head, key, o);
+                fa_after();
+                const bool bad = R->bad != 0;
                 const long long at = (long long)w.row0 * a.ld + head * kHeadDim + key;
                 // Record 2 c of a piece that began before this CTA's range, 2 c + 1 of one that begins in it.
                 float* rec = a.part + ((long long)(2 * c + (w.begins ? 1 : 0)) * a.heads + head) * NR * kPartStride;
+                // Rolled: code that runs once a piece costs more to fetch than to run.
+#pragma unroll 1
+                for (int g = 0; g < groups; ++g) {
+                    float o[16];
+                    ld16(lanes + 64 + 16 * g, o);
+                    fa_wait_ld();
+                    if (bad) add_not_finite(a, *R, w, base_slot, head, key, 16 * g, o);
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    if (g >= groups) continue;
-                    if (w.whole) {
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const int r = 16 * g + j;
-                            const float y = o[r] * R->sum[r];
-                            if (r < w.nrows) {
-                                if constexpr (P2) static_cast<float*>(a.out)[at + (long long)r * a.ld] = y;
-                                else static_cast<__nv_bfloat16*>(a.out)[at + (long long)r * a.ld] = __float2bfloat16_rn(y);
-                            }
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (16 * g + j < w.nrows) rec[(16 * g + j) * kPartStride + key] = o[16 * g + j];
+                    for (int j = 0; j < 16; ++j) {
+                        const int r = 16 * g + j;
+                        if (r >= w.nrows) continue;
+                        if (!w.whole) rec[r * kPartStride + key] = o[j];
+                        else if constexpr (P2) static_cast<float*>(a.out)[at + (long long)r * a.ld] = o[j] * R->sum[r];
+                        else static_cast<__nv_bfloat16*>(a.out)[at + (long long)r * a.ld] = __float2bfloat16_rn(o[j] * R->sum[r]);
                     }
                 }
+                fa_before();  // O is read before the next piece's first P V (through pfull)
                 if (!w.whole && key < w.nrows)
-                    *reinterpret_cast<float2*>(rec + key * kPartStride + NR) = make_float2(BOUNDED || R->has[key] ? R->m[key] : kScoreLow, R->sum[key]);
+                    *reinterpret_cast<float2*>(rec + key * kPartStride + NR) =
+                        make_float2(BOUNDED || R->has[key] ? R->m[key] : kScoreLow, R->sum[key]);
             }
             head_any(hl, false);  // the rows' arrays are the next block's from here
         }
@@ -497,17 +514,17 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
             const uint32_t rows = (uint32_t)((w.nrows + 15) / 16 * 16);
             for (int it = 0; it < n && ok; ++it, ++i) {
                 // S goes first where its keys are there; else P V of the item before, then S.
-                const bool there = i == 0 || (it > 0 && mbar_test_wait(k_full(i), (i / kSlots) & 1));
+                const bool there = it == 0 || mbar_test_wait(k_full(i), (i / kSlots) & 1);
                 if (!there) pv_before();
                 ok = ok && mbar_wait(k_full(i), (i / kSlots) & 1) && mbar_wait(&b->qready, piece & 1) &&
                      (i == 0 || mbar_wait(&b->sfree, (i - 1) & 1));
                 if (ok) issue_s(i, rows, it == n - 1);
-                if (there && i > 0) pv_before();
+                if (there && it > 0) pv_before();
                 last_rows = rows;
                 last_first = it == 0;
             }
+            pv_before();  // the piece's last
         }
-        if (i > 0) pv_before();
         if (!ok) set_error(a.err, DEV_ERR_TIMEOUT);
       } else if (warp == 10 && lane == 0 && !idle) {
         // ---- producer -------------------------------------------------------------------------------
