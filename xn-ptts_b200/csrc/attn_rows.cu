@@ -30,6 +30,8 @@
 // itself is rounded. An item that some row does not see whole has a bit per row in each key's thread, and
 // takes values that are not finite out of the V tile (0 x NaN is NaN); rows that see such a value get it
 // back at the piece's end, from the cache.
+#include <type_traits>
+
 #include "common.cuh"
 #include "fa_tc.cuh"
 #include "score.cuh"
@@ -444,13 +446,22 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
                     ld16(lanes + 64 + 16 * g, o);
                     fa_wait_ld();
                     if (bad) add_not_finite(a, *R, w, base_slot, head, key, 16 * g, o);
+const int rows = w.nrows - 16 * g;  // of these 16
+                    if (w.whole) {
+                        using Out = typename std::conditional<P2, float, __nv_bfloat16>::type;
+                        Out* out = static_cast<Out*>(a.out) + at + (long long)(16 * g) * a.ld;
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int r = 16 * g + j;
-                        if (r >= w.nrows) continue;
-                        if (!w.whole) rec[r * kPartStride + key] = o[j];
-                        else if constexpr (P2) static_cast<float*>(a.out)[at + (long long)r * a.ld] = o[j] * R->sum[r];
-                        else static_cast<__nv_bfloat16*>(a.out)[at + (long long)r * a.ld] = __float2bfloat16_rn(o[j] * R->sum[r]);
+                        for (int j = 0; j < 16; j += 4) {
+                            const float4 f = *reinterpret_cast<const float4*>(&R->sum[16 * g + j]);
+                            o[j] *= f.x, o[j + 1] *= f.y, o[j + 2] *= f.z, o[j + 3] *= f.w;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (j < rows) out[j * a.ld] = from_f32<Out>(o[j]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (j < rows) rec[(16 * g + j) * kPartStride + key] = o[j];
                     }
                 }
                 fa_before();  // O is read before the next piece's first P V (through pfull)
