@@ -766,7 +766,6 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
         // CTAs still get two or more to even out.
         a.heads_per_cta = kGroupHeads;
         while (a.heads_per_cta > 1 && (long long)a.n_tiles * (kv->heads / a.heads_per_cta) < 4LL * grid) a.heads_per_cta /= 2;
-        if (getenv("HPC")) a.heads_per_cta = atoi(getenv("HPC"));
         a.err = p.err;
         require(launch_score_prompt(a, s), PTTS_B200_ERR_CUDA,
                 "could not describe the prompt attention's tensors (cuTensorMapEncodeTiled)");

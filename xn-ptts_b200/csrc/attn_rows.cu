@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
                     }
                     if (!whole) {
                         ok = __all_sync(0xffffffffu, mbar_wait(&b->vfull[i % kSlots], (i / kSlots) & 1));
-                        if (ok) clean_v(sm + L::kV + (hl * kSlots + i % kSlots) * kTile, key, (seen[0] | seen[1]) == 0, &R->bad);
+                        if (ok) clean_v<8>(sm + L::kV + (hl * kSlots + i % kSlots) * kTile, key, 0, (seen[0] | seen[1]) == 0, &R->bad);
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // P, and V where it was cleaned
                     fa_before();

@@ -14,7 +14,7 @@
 //              in two-slot rings, so the next head's data come during this head's last item.
 // Two threads a row and two CTAs an SM make four softmax warps a scheduler, which fill each other's
 // waits (with a thread a row, half as many, the issue slots were 35 to 46 % used). Where a cap up to
-// kBoundedCap bounds the scores there is no maximum: exp2 runs against the bias of the row's nearest
+// kScoreBoundedCap bounds the scores there is no maximum: exp2 runs against the bias of the row's nearest
 // key, which a score passes by at most cap x log2(e) < 58 either way. Items run from the last keys to
 // the first: a causal row's nearest keys, whose bias is the least, set the maximum at once.
 //
@@ -35,15 +35,14 @@ namespace ptts {
 namespace {
 
 constexpr int QT = 128, KT = 128;
-constexpr int kSoftW = 4, kMmaW = kSoftW, kLoadW = kSoftW + 1;
-// Two warpgroups: the softmax takes most of the launch's 256 x 128 registers (128 scores a thread).
-constexpr int kThreadsP = 256, kRegsP = 128, kRegsSoft = 200, kRegsRest = 56;
-static_assert(128 * (kRegsSoft + kRegsRest) <= kThreadsP * kRegsP, "the split fits the launch");
+constexpr int kSoftW = 8, kMmaW = kSoftW, kLoadW = kSoftW + 1, kThreadsP = (kSoftW + 2) * 32;
 constexpr int kTile = 128 * 128;  // bytes of a Q plane, a K tile or a V tile: 128 rows x 64 bf16
 constexpr int kSlots = 2;
 constexpr int kOffK = 2 * kTile, kOffV = kOffK + kSlots * kTile, kOffBars = kOffV + kSlots * kTile;
-constexpr int kSmemP = 1024 + kOffBars + 256;
-static_assert(2 * (kSmemP + 1024 + 1024) <= 228 * 1024, "two CTAs per SM");
+constexpr int kOffKx = kOffBars + 1024, kOffQx = kOffKx + 4096;  // the bias operands: 128 rows of 16 bf16 each
+constexpr int kSmemP = 1024 + kOffQx + 4096;
+constexpr int kStaticP = 4608;  // s_xmax, s_xsum and the small ones
+static_assert(2 * (kSmemP + kStaticP + 1024) <= 228 * 1024, "two CTAs per SM");
 constexpr uint32_t kCols = 256, kColS = 0, kColO = 128, kColP = 192;
 constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((KT / 8) << 17) | (8u << 24);
 constexpr uint32_t kIdescPV = (1u << 4) | (1u << 7) | (1u << 10) | (8u << 17) | (8u << 24) | (1u << 16);
@@ -56,7 +55,6 @@ struct Bars {
     uint64_t qready, kfull[kSlots], kempty[kSlots], vfull[kSlots], vempty[kSlots], qfree, sfull, sfree, pfull, odone;
 };
 
-
 // The values of slots lo .. hi that are not finite, from the cache, onto 32 dims of a row.
 __device__ __forceinline__ void add_not_finite(const ScorePromptArgs& a, int kv_row, int x, int lo, int hi, float* o) {
     const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.v_cache) + ((long long)kv_row + lo) * kRowWidth + x;
@@ -68,40 +66,53 @@ __device__ __forceinline__ void add_not_finite(const ScorePromptArgs& a, int kv_
         }
 }
 
-// 32 scores of a row: capped, biased (`ahead` = position - first key), -inf outside keys from .. to
-// (unless `whole`: every key is visible).
+// Named barrier 1 + quarter over the two softmax warps of 32 rows: whether `v` held in any thread.
+__device__ __forceinline__ bool pair_any(int quarter, bool v) {
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred q, %2, 64, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any)
+        : "r"((uint32_t)v), "r"(1 + quarter)
+        : "memory");
+    return any != 0;
+}
+// K-major, 32-byte swizzle (8-row groups 256 B apart): the bias operands.
+__device__ __forceinline__ uint64_t desc_x(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)1u << 16) | ((uint64_t)(256 >> 4) << 32) |
+           ((uint64_t)1u << 46) | ((uint64_t)6u << 61);
+}
+// Row r of a bias operand: three values, then zeros.
+__device__ __forceinline__ void put_x(unsigned char* x, int r, uint32_t v01, uint32_t v2) {
+    uint4* row = reinterpret_cast<uint4*>(x + 32 * r);
+    row[r >> 2 & 1] = make_uint4(v01, v2, 0u, 0u);
+    row[(r >> 2 & 1) ^ 1] = make_uint4(0u, 0u, 0u, 0u);
+}
+
+// 32 scores of a row: capped, biased (`ahead` = position - first key), -inf where `seen` has no bit.
+// Without a cap the products have added slope x (key's place in the item) already, which is the bias up to
+// a constant per row as long as no visible key is ahead of the row; `over`: some may be.
 template <int CAP, bool BIAS>
-__device__ __forceinline__ void rules(float* s, float cap, float slope, int ahead, int from, int to, bool whole) {
+__device__ __forceinline__ void rules(float* s, float cap, float slope, int ahead, bool over, uint32_t seen) {
     if (CAP == kCapFast) cap_fast<32>(s, cap);
     if (CAP == kCapExact) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) s[j] = cap_exact(s[j], cap);
     }
-    if (BIAS && __all_sync(0xffffffffu, ahead >= 31)) {  // no key ahead of its row: slope j - slope ahead
-        const float at = -slope * (float)ahead;
-        const float2 at2 = make_float2(at, at);
-#pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-            const float2 t = __fadd2_rn(make_float2(s[j], s[j + 1]), at2);
-            s[j] = fmaf(slope, (float)j, t.x);
-            s[j + 1] = fmaf(slope, (float)(j + 1), t.y);
-        }
-    } else if (BIAS) {
+    if (BIAS && CAP != kCapNone) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) s[j] = fmaf(-slope, fabsf((float)ahead - (float)j), s[j]);
     }
-    if (!whole && __any_sync(0xffffffffu, from > 0 || to < 31)) {
-        const uint32_t x = from <= 0 ? 0xffffffffu : (from > 31 ? 0u : 0xffffffffu << from);
-        const uint32_t y = to >= 31 ? 0xffffffffu : (to < 0 ? 0u : 0xffffffffu >> (31 - to));
+    if (BIAS && CAP == kCapNone && over) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) s[j] = (x & y) >> j & 1 ? s[j] : -INFINITY;
+        for (int j = 0; j < 32; ++j) s[j] = fmaf(-2.f * slope, fmaxf((float)j - (float)ahead, 0.f), s[j]);
     }
-}
-// The item's scores are in this warp's registers: S may take the next item's.
-__device__ __forceinline__ void s_is_read(Bars* b, int lane) {
-    fa_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&b->sfree);
+    if (__any_sync(0xffffffffu, seen != 0xffffffffu)) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) s[j] = seen >> j & 1 ? s[j] : -INFINITY;
+    }
 }
 __device__ __forceinline__ float most_of(const float* s) {  // four chains of three-input maxima
     float m[4];
@@ -139,11 +150,15 @@ __global__ void __launch_bounds__(kThreadsP, 2) score_prompt_kernel(ScorePromptA
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     unsigned char* sm = smem_raw + (base - raw);
     Bars* b = reinterpret_cast<Bars*>(sm + kOffBars);
+    // Without a cap the bias comes out of the products: S += Qx Kx^T with the slope, as three bf16 parts
+    // of its 24 bits, against the key's place in the item (exact in bf16), one MMA step of 16.
+    constexpr bool kBiasMma = BIAS && CAP == kCapNone;
     __shared__ uint32_t s_tmem;
+    __shared__ float s_xmax[2][2][QT], s_xsum[2][2][QT];  // [item or head parity][half][row]
     __shared__ int s_lo[4], s_hi[4], s_lo_most[4], s_hi_least[4], s_bad, s_q_issued, s_k_issued, s_v_issued;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        mbar_init(&b->qready, 1);
+        mbar_init(&b->qready, kBiasMma ? 2 : 1);  // the copies, and the slope
         for (int i = 0; i < kSlots; ++i) {
             mbar_init(&b->kfull[i], 1);
             mbar_init(&b->kempty[i], 1);
@@ -163,6 +178,11 @@ __global__ void __launch_bounds__(kThreadsP, 2) score_prompt_kernel(ScorePromptA
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    if (kBiasMma && tid < KT) {
+        const float j = (float)tid;
+        put_x(sm + kOffKx, tid, pack_bf16x2(j, j), pack_bf16x2(j, 0.f));
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
     grid_dep_wait();
     grid_dep_launch();
     const int slabs = a.heads / a.heads_per_cta, head0 = blockIdx.x % slabs * a.heads_per_cta;
@@ -171,14 +191,14 @@ __global__ void __launch_bounds__(kThreadsP, 2) score_prompt_kernel(ScorePromptA
     // The row of each softmax thread, and the slots the tile's rows see: any (min lo .. max hi) and
     // all (max lo .. min hi).
     int lo = 0, hi = -1;
-    const int r = tid;  // softmax threads: row r
+    const int r = 32 * (warp & 3) + lane, half = warp >> 2;  // softmax threads: row r, keys 64 half ..
     const bool there = r < nrows;
     if (warp < kSoftW) {
         if (there) lo = a.rows.lo[row0 + r], hi = a.rows.hi[row0 + r];
         const bool sees = lo <= hi;
         const int x0 = __reduce_min_sync(0xffffffffu, sees ? lo : 0x7fffffff), x1 = __reduce_max_sync(0xffffffffu, sees ? hi : -1);
         const int y0 = __reduce_max_sync(0xffffffffu, there ? lo : 0), y1 = __reduce_min_sync(0xffffffffu, there ? hi : 0x7fffffff);
-        if (lane == 0) s_lo[warp] = x0, s_hi[warp] = x1, s_lo_most[warp] = y0, s_hi_least[warp] = y1;
+        if (lane == 0 && half == 0) s_lo[warp] = x0, s_hi[warp] = x1, s_lo_most[warp] = y0, s_hi_least[warp] = y1;
     }
     fa_before();
     __syncthreads();
@@ -198,8 +218,7 @@ __global__ void __launch_bounds__(kThreadsP, 2) score_prompt_kernel(ScorePromptA
     auto kv_x = [&](int head) { return (head % kGroupHeads) * kHeadDim; };
 
     if (warp < kSoftW) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoft));
-        const uint32_t lanes = tmem + ((uint32_t)(32 * warp) << 16);
+        const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const int pos = BIAS && there ? a.rows.pos[row0 + r] : 0;
         const float2 minus1 = make_float2(-1.f, -1.f);
         float m = 0.f, l = 0.f, slope = 0.f;
@@ -208,153 +227,180 @@ __global__ void __launch_bounds__(kThreadsP, 2) score_prompt_kernel(ScorePromptA
             float o[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) o[j] = 0.f;
-            for (int hh = 0; hh < a.heads_per_cta; ++hh) {
-                store_half<P2>(a, row0 + r, head0 + hh, 0, o);
-                store_half<P2>(a, row0 + r, head0 + hh, 1, o);
-            }
+            for (int hh = 0; hh < a.heads_per_cta; ++hh) store_half<P2>(a, row0 + r, head0 + hh, half, o);
         }
-        for (int i = 0, kt = 0, head = head0; i < items; ++i) {
+        // A wait that gives up clears `ok`; the row's other half learns of it at the next barrier they
+        // share (per item, or BOUNDED per head), and both leave there.
+        for (int i = 0, kt = 0, hh = 0; i < items; ++i) {
+            const int head = head0 + hh;
             if (kt == 0) {
                 if (BIAS) slope = a.rule.slopes[head] * kScoreLog2e;
                 // BOUNDED: exp2 against the bias of the nearest visible key.
                 m = BOUNDED ? (BIAS ? -slope * (float)max(max(lo - pos, pos - hi), 0) : 0.f) : kScoreLow;
                 l = 0.f;
             }
-            const int k0 = first + (n - 1 - kt) * KT;
-            ok = __all_sync(0xffffffffu, mbar_wait(&b->sfull, i & 1));
-            if (!ok) break;
-            fa_after();
-            // Whether some row of the warp sees some of each 32 keys; every row every key: `whole`.
-            const bool whole = k0 >= lo_most && k0 + KT - 1 <= hi_least;
-            uint32_t alive = 0xfu;
+            const int k0 = first + (n - 1 - kt) * KT, mine = k0 + 64 * half;  // this thread's first key
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(&b->sfull, i & 1));
+            // The scores are taken 32 at a time, for the maximum and again for P (capped ones go back to
+            // TMEM in between): all 64 in registers spill, which cost more than the second read.
+            float mt = -INFINITY;
+            const bool whole = k0 >= lo_most && k0 + KT - 1 <= hi_least;  // every row sees every key
+            uint32_t seen[2] = {~0u, ~0u};  // this row's visible keys, a bit each
+            bool alive[2] = {true, true};   // whether some row of the warp sees some of the 32 keys
             if (!whole) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (!__any_sync(0xffffffffu, lo <= k0 + 32 * c + 31 && hi >= k0 + 32 * c)) alive &= ~(1u << c);
+                for (int c = 0; c < 2; ++c) {
+                    const int x = lo - mine - 32 * c, y = hi - mine - 32 * c;  // bits x .. y
+                    const uint32_t from = x <= 0 ? 0xffffffffu : (x > 31 ? 0u : 0xffffffffu << x);
+                    const uint32_t to = y >= 31 ? 0xffffffffu : (y < 0 ? 0u : 0xffffffffu >> (31 - y));
+                    seen[c] = from & to;
+                    alive[c] = __any_sync(0xffffffffu, seen[c] != 0);
+                }
             }
-            float s[BOUNDED ? 32 : KT];
-            bool waited = i == 0;  // for P V of the item before
-            if (!BOUNDED) {
+            const bool over = kBiasMma && __any_sync(0xffffffffu, min(hi, mine + 63) > pos);
+            const float bias = kBiasMma ? slope * (float)(k0 - pos) : 0.f;  // the products' bias is slope x (key - k0)
+            if (ok) fa_after();
+            if (!BOUNDED && ok) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) fa_ld32(lanes + kColS + 32 * c, s + 32 * c);
-                fa_wait_ld();
-                if (!P2) s_is_read(b, lane);
-                float mt = -INFINITY;
+                for (int c = 0; c < 2; ++c) {
+                    if (alive[c]) {
+                        float s[32];
+                        const uint32_t at = lanes + kColS + 64 * half + 32 * c;
+                        fa_ld32(at, s);
+                        fa_wait_ld();
+                        rules<CAP, BIAS>(s, a.rule.cap, slope, pos - mine - 32 * c, over, seen[c]);
+                        mt = fmaxf(mt, most_of(s) + bias);
+                        if (CAP != kCapNone) {
+                            uint32_t w[32];
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (alive >> c & 1) {
-                        rules<CAP, BIAS>(s + 32 * c, a.rule.cap, slope, pos - k0 - 32 * c, lo - k0 - 32 * c, hi - k0 - 32 * c, whole);
-                        mt = fmaxf(mt, most_of(s + 32 * c));
+                            for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(s[j]);
+                            fa_st32(at, w);
+                            wait_st();
+                        }
                     }
+                }
+            }
+            bool waited = i == 0;  // for P V of the item before
+            // One barrier of the two warps of 32 rows: unless a score of theirs passed m by more than
+            // kRaiseP (or a wait gave up), m stays and nothing is exchanged.
+            if (!BOUNDED && pair_any(warp & 3, !ok || mt > m + kRaiseP)) {
+                s_xmax[i & 1][half][r] = mt;
+                if (pair_any(warp & 3, !ok)) break;
+                mt = fmaxf(mt, s_xmax[i & 1][half ^ 1][r]);
                 const bool raise = mt > m + kRaiseP;
-                if (__any_sync(0xffffffffu, raise)) {
-                    const float mn = raise ? mt : m, f = score_exp2(m - mn);
-                    l *= f;
-                    m = mn;
-                    if (kt > 0) {  // O holds the head's items before this one once their P V is done
-                        ok = __all_sync(0xffffffffu, mbar_wait(&b->odone, (i - 1) & 1));
-                        if (!ok) break;
-                        waited = true;
+                const float mn = raise ? mt : m, f = score_exp2(m - mn);
+                l *= f;
+                m = mn;
+                if (kt > 0) {  // O holds the head's items before this one once their P V is done
+                    ok = __all_sync(0xffffffffu, mbar_wait(&b->odone, (i - 1) & 1));
+                    waited = true;
+                    if (ok) {
                         fa_after();
 #pragma unroll 1
-                        for (int c = 0; c < 8; ++c) {
+                        for (int c = 0; c < 4; ++c) {
                             float o[8];
                             uint32_t w[8];
-                            ld8(lanes + kColO + 8 * c, o);
+                            ld8(lanes + kColO + 32 * half + 8 * c, o);
                             fa_wait_ld();
 #pragma unroll
                             for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(o[j] * f);
-                            fa_st8(lanes + kColO + 8 * c, w);
+                            fa_st8(lanes + kColO + 32 * half + 8 * c, w);
                         }
                         wait_st();
                     }
                 }
             }
-            if (!P2 && !waited) {  // P V of the item before has read P
+            if (!P2 && ok && !waited) {  // P V of the item before has read P
                 ok = __all_sync(0xffffffffu, mbar_wait(&b->odone, (i - 1) & 1));
-                if (!ok) break;
                 fa_after();
             }
-            // P, 32 keys at a time: bf16 pairs into its own columns, or (P2) hi and lo over the 32
-            // columns of S they came from.
-            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-            const float2 neg_m = make_float2(-m, -m);
+            if (ok) {
+                // P, 32 keys at a time: bf16 pairs into its own columns, or (P2) hi and lo over the 32
+                // columns of S they came from.
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                const float2 neg_m = make_float2(bias - m, bias - m);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t ph[16], pl[P2 ? 16 : 1];
-                float* sc = s + (BOUNDED ? 0 : 32 * c);
-                if (BOUNDED && (alive >> c & 1)) {
-                    fa_ld32(lanes + kColS + 32 * c, sc);
-                    fa_wait_ld();
-                }
-                if (BOUNDED && !P2 && c == 3) s_is_read(b, lane);
-                if (alive >> c & 1) {
-                    if (BOUNDED) rules<CAP, BIAS>(sc, a.rule.cap, slope, pos - k0 - 32 * c, lo - k0 - 32 * c, hi - k0 - 32 * c, whole);
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t ph[16], pl[P2 ? 16 : 1];
+                    float s[32];
+                    if (alive[c]) {
+                        fa_ld32(lanes + kColS + 64 * half + 32 * c, s);
+                        fa_wait_ld();
+                    }
+                    if (!P2 && c == 1) {  // the scores are read: S may take the next item's
+                        fa_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&b->sfree);
+                    }
+                    if (alive[c]) {
+                        if (BOUNDED || CAP == kCapNone)
+                            rules<CAP, BIAS>(s, a.rule.cap, slope, pos - mine - 32 * c, over, seen[c]);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        float2 x = make_float2(sc[2 * j], sc[2 * j + 1]);
-                        if (!BOUNDED || BIAS) x = __fadd2_rn(x, neg_m);
-                        const float2 e = make_float2(score_exp2(x.x), score_exp2(x.y));
-                        sum[j & 1] = __fadd2_rn(sum[j & 1], e);
-                        ph[j] = pack_bf16x2(e.x, e.y);
-                        if constexpr (P2) {
-                            const float2 d = __ffma2_rn(make_float2(bf16lo(ph[j]), bf16hi(ph[j])), minus1, e);
-                            pl[j] = pack_bf16x2(d.x, d.y);
+                        for (int j = 0; j < 16; ++j) {
+                            float2 x = make_float2(s[2 * j], s[2 * j + 1]);
+                            if (!BOUNDED || BIAS) x = __fadd2_rn(x, neg_m);
+                            const float2 e = make_float2(score_exp2(x.x), score_exp2(x.y));
+                            sum[j & 1] = __fadd2_rn(sum[j & 1], e);
+                            ph[j] = pack_bf16x2(e.x, e.y);
+                            if constexpr (P2) {
+                                const float2 d = __ffma2_rn(make_float2(bf16lo(ph[j]), bf16hi(ph[j])), minus1, e);
+                                pl[j] = pack_bf16x2(d.x, d.y);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            ph[j] = 0u;
+                            if constexpr (P2) pl[j] = 0u;
                         }
                     }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        ph[j] = 0u;
-                        if constexpr (P2) pl[j] = 0u;
+                    if constexpr (P2) {
+                        st16(lanes + kColS + 64 * half + 32 * c, ph);
+                        st16(lanes + kColS + 64 * half + 32 * c + 16, pl);
+                    } else {
+                        st16(lanes + kColP + 32 * half + 16 * c, ph);
                     }
                 }
-                if constexpr (P2) {
-                    st16(lanes + kColS + 32 * c, ph);
-                    st16(lanes + kColS + 32 * c + 16, pl);
-                } else {
-                    st16(lanes + kColP + 16 * c, ph);
+                l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
+                wait_st();
+                if (!whole) {
+                    // Some row does not see some key: half a key's V row a thread, cleaned in shared memory.
+                    ok = __all_sync(0xffffffffu, mbar_wait(&b->vfull[i % kSlots], (i / kSlots) & 1));
+                    if (ok) clean_v<4>(sm + kOffV + (i % kSlots) * kTile, tid >> 1, 4 * (tid & 1), k0 + (tid >> 1) >= end, &s_bad);
                 }
-            }
-            l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
-            wait_st();
-            if (!whole) {  // some row does not see some key: a V row a thread, cleaned in shared memory
-                ok = __all_sync(0xffffffffu, mbar_wait(&b->vfull[i % kSlots], (i / kSlots) & 1));
-                if (!ok) break;
-                clean_v(sm + kOffV + (i % kSlots) * kTile, tid, k0 + tid >= end, &s_bad);
-            }
-            fa_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&b->pfull);
-            if (++kt < n) continue;
-            // The head's end: O / l to the output. P V done also means that every warp's s_bad is seen
-            // (they wrote it before their arrivals on pfull).
-            ok = __all_sync(0xffffffffu, mbar_wait(&b->odone, i & 1));
-            if (!ok) break;
-            fa_after();
-            const bool bad = *const_cast<volatile int*>(&s_bad) != 0;
-            const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float o[32];
-                fa_ld32(lanes + kColO + 32 * c, o);
-                fa_wait_ld();
-                if (there) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) o[j] *= inv;
-                    if (bad) add_not_finite(a, kv_row(head), kv_x(head) + 32 * c, lo, hi, o);
-                    store_half<P2>(a, row0 + r, head, c, o);
-                }
+                fa_before();
                 __syncwarp();
+                if (lane == 0) mbar_arrive(&b->pfull);
             }
+            if (++kt < n) continue;
+            // The head's end: O / l, the sum over both halves, to the output. P V done also means that
+            // every warp's s_bad is seen (they wrote it before their arrivals on pfull).
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(&b->odone, i & 1));
+            s_xsum[hh & 1][half][r] = l;
+            if (pair_any(warp & 3, !ok)) {
+                ok = false;
+                break;
+            }
+            fa_after();
+            l += s_xsum[hh & 1][half ^ 1][r];
+            const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
+            float o[32];
+            ld16(lanes + kColO + 32 * half, o);
+            ld16(lanes + kColO + 32 * half + 16, o + 16);
+            fa_wait_ld();
             fa_before();  // O is read before the next head's first P V (through pfull)
+            if (there) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) o[j] *= inv;
+                if (*const_cast<volatile int*>(&s_bad)) add_not_finite(a, kv_row(head), kv_x(head) + 32 * half, lo, hi, o);
+                store_half<P2>(a, row0 + r, head, half, o);
+            }
+            __syncwarp();
             kt = 0;
-            ++head;
+            ++hh;
         }
         if (!ok && lane == 0) set_error(a.err, DEV_ERR_TIMEOUT);
-    } else {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
-      if (warp == kMmaW && lane == 0) {
+    } else if (warp == kMmaW && lane == 0) {
         // ---- MMA issuer ------------------------------------------------------------------------
         auto issue_s = [&](int i) {
             fa_after();
@@ -364,6 +410,7 @@ __global__ void __launch_bounds__(kThreadsP, 2) score_prompt_kernel(ScorePromptA
                 fa_mma_ss(tmem + kColS, qh + 2 * k, dk + 2 * k, kIdescS, k ? 1u : 0u);
                 fa_mma_ss(tmem + kColS, ql + 2 * k, dk + 2 * k, kIdescS, 1u);
             }
+            if (kBiasMma) fa_mma_ss(tmem + kColS, desc_x(base + kOffQx), desc_x(base + kOffKx), kIdescS, 1u);
             fa_commit(&b->sfull);
             fa_commit(&b->kempty[i % kSlots]);
             if (i % n == n - 1) fa_commit(&b->qfree);  // the head's last use of Q
@@ -404,6 +451,13 @@ __global__ void __launch_bounds__(kThreadsP, 2) score_prompt_kernel(ScorePromptA
                 fa_tma(base, &tm_qh, head * kHeadDim, row0, &b->qready);
                 fa_tma(base + kTile, &tm_ql, head * kHeadDim, row0, &b->qready);
                 s_q_issued = hh + 1;
+                if (kBiasMma) {  // the head's slope in three parts, for every row
+                    const float slope = a.rule.slopes[head] * kScoreLog2e;
+                    const float p0 = __bfloat162float(__float2bfloat16_rn(slope)), p1 = __bfloat162float(__float2bfloat16_rn(slope - p0));
+                    for (int q = 0; q < QT; ++q) put_x(sm + kOffQx, q, pack_bf16x2(p0, p1), pack_bf16x2(slope - p0 - p1, 0.f));
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    mbar_arrive(&b->qready);
+                }
             }
             if (i >= kSlots && !(ok = mbar_wait(&b->kempty[slot], ((i / kSlots) & 1) ^ 1))) break;
             mbar_arrive_expect_tx(&b->kfull[slot], kTile);
@@ -416,7 +470,6 @@ __global__ void __launch_bounds__(kThreadsP, 2) score_prompt_kernel(ScorePromptA
             if (++kt == n) kt = 0, ++hh;
         }
         if (!ok) set_error(a.err, DEV_ERR_TIMEOUT);
-      }
     }
     fa_before();
     __syncthreads();

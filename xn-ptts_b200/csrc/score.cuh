@@ -79,33 +79,38 @@ __device__ __forceinline__ bool drop_not_finite(uint32_t& u) {
     return lo || hi;
 }
 
-// Key `key` of a V tile: zeros if the key is gone, else without what is not finite
-// (x 0 is NaN then), which `bad` records. Swizzled 16-byte chunks; visible to the products afterwards.
-__device__ __forceinline__ void clean_v(unsigned char* tile, int key, bool gone, int* bad) {
+// 16-byte chunks c0 .. c0 + N - 1 of key `key` in a V tile: zeros if the key is gone, else without what is
+// not finite (x 0 is NaN then), which `bad` records. Swizzled 16-byte chunks; visible to the products
+// afterwards.
+template <int N>
+__device__ __forceinline__ void clean_v(unsigned char* tile, int key, int c0, bool gone, int* bad) {
     uint4* v = reinterpret_cast<uint4*>(tile + key * 128);
     const uint32_t zero = 0;
     uint32_t probe = 0;
-    uint4 w[8];
+    uint4 w[N];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-        w[c] = v[c ^ (key & 7)];
+    for (int c = 0; c < N; ++c) {
+        w[c] = v[(c0 + c) ^ (key & 7)];
         const uint32_t* u = &w[c].x;
 #pragma unroll
         for (int j = 0; j < 4; ++j) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(probe) : "r"(u[j]), "r"(zero));
     }
     const bool drop = (probe & 0x7fff7fffu) != 0;  // NaN in either half
     if (gone || drop) {
+        if (!gone) {  // recorded first: whoever reads the cleaned row finds the record
+            *bad = 1;
+            __threadfence_block();
+        }
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
+        for (int c = 0; c < N; ++c) {
             uint32_t* u = &w[c].x;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (gone) u[j] = 0u;
                 else drop_not_finite(u[j]);
             }
-            v[c ^ (key & 7)] = w[c];
+            v[(c0 + c) ^ (key & 7)] = w[c];
         }
-        if (!gone) *bad = 1;
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }

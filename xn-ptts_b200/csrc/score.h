@@ -122,8 +122,8 @@ int score_rows_grid(bool out_bf16, int heads, int sms);  // CTAs along the keys 
 size_t score_rows_part_floats(int heads, int grid);
 bool launch_score_rows(const ScoreRowsArgs& a, int grid, cudaStream_t s);
 
-// Prompts on tcgen05, bf16 caches (attn_score_prompt.cu): tiles (first row, rows) of up to 128 rows
-// of one sequence. False: the tensor maps could not be made, nothing launched.
+// Prompts on tcgen05, bf16 caches (attn_score_prompt.cu): tiles (first row, rows) of up to 128
+// rows of one sequence. False: the tensor maps could not be made, nothing launched.
 struct ScorePromptArgs {
     const void* k_cache;  // the layer
     const void* v_cache;
