@@ -620,14 +620,19 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
     refuse_capture(s, tree ? "ptts_b200_attend_tree" : "ptts_b200_attend_scored");
     const bool cache_bf16 = kv->dtype == PTTS_B200_BF16;
     const size_t hd = (size_t)kv->heads * kHeadDim;
-    // Single tokens run on the split-KV decode, a row per unit; up to 64 rows a sequence on a bf16
-    // cache in blocks of rows, split over the keys; longer prompts in tiles of 128 rows.
+    // Single tokens run on the split-KV decode, a row per unit. On a bf16 cache up to 64 rows a sequence
+    // run as blocks split over the keys, longer prompts in tiles of 128 rows; on an f32 cache both in
+    // tiles of 32 rows.
     const int most = *std::max_element(rows_host, rows_host + n_seq);
     const bool tokens = !tree && n_rows == n_seq, few = !tokens && cache_bf16 && most <= kTreeNodes;
     const bool prompt = !tokens && cache_bf16 && !few, out_bf16 = out_dtype == PTTS_B200_BF16;
     int grid = sm_count(kv->device);
     std::vector<int2> blocks;
     if (prompt) blocks = make_tiles(offsets, streams_host, kv->h_len);
+    if (!tokens && !cache_bf16)
+        for (int i = 0; i < n_seq; ++i)
+            for (int r = offsets[i]; r < offsets[i + 1]; r += kScoreF32Rows)
+                blocks.push_back(make_int2(r, std::min(kScoreF32Rows, offsets[i + 1] - r)));
     if (few) {
         grid = score_rows_grid(out_bf16, kv->heads, grid);
         for (int i = 0; i < n_seq; ++i) blocks.push_back(make_int2(offsets[i], rows_host[i]));
@@ -772,12 +777,12 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
         check_launch();
         return;
     }
-    ScoreCoreArgs a{};
+    ScoreF32Args a{};
     a.k_cache = p.k_cache;
     a.v_cache = p.v_cache;
     a.q = p.q_out;
     a.out = out;
-    a.out_bf16 = out_dtype == PTTS_B200_BF16;
+    a.out_bf16 = out_bf16;
     a.n_rows = n_rows;
     a.heads = kv->heads;
     a.num_streams = kv->streams;
@@ -785,8 +790,14 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
     a.rows = p.rows;
     a.rule.cap = sc.softcap;
     a.rule.slopes = sc.slopes;
-    a.err = p.err;
-    launch_score_core(a, cache_bf16, s);
+    a.tiles = reinterpret_cast<const int2*>(d + blocks_at);
+    a.n_tiles = (int)blocks.size();
+    int most_keys = 0;
+    for (int i = 0; i < n_seq; ++i) most_keys = std::max(most_keys, kv->h_len[streams_host[i]] + rows_host[i]);
+    a.splits = score_f32_splits(a.n_tiles, kv->heads, most_keys, grid);
+    if (a.splits > 1)
+        a.part = static_cast<float*>(kv->part.need(sizeof(float) * kPartStride * a.splits * kv->heads * (size_t)n_rows));
+    launch_score_f32(a, s);
     check_launch();
 }
 

@@ -68,8 +68,10 @@ struct ScorePlanArgs {
 // One launch: every row's plan entry, its rotated q, its cache rows; and the units' partition.
 void launch_score_plan(const ScorePlanArgs& a, bool in_bf16, bool cache_bf16, cudaStream_t s);
 
-// Attention on CUDA cores, one warp per (row, head), any cache type.
-struct ScoreCoreArgs {
+// Prompts and trees on f32 caches (attn_score_f32.cu): tiles (first row, rows) of up to kScoreF32Rows rows
+// of one sequence; with splits > 1 the tiles' keys are shared out and joined through `part`.
+constexpr int kScoreF32Rows = 32;
+struct ScoreF32Args {
     const void* k_cache;  // the layer: kv_offset's layout
     const void* v_cache;
     const float* q;       // [n_rows][H * 64] f32, rotated
@@ -78,9 +80,13 @@ struct ScoreCoreArgs {
     int n_rows, heads, num_streams, capacity;
     ScoreRows rows;
     ScoreRule rule;
-    uint32_t* err;
+    const int2* tiles;
+    int n_tiles;
+    int splits;
+    float* part;          // [n_rows][H][splits][kPartStride] with splits > 1
 };
-void launch_score_core(const ScoreCoreArgs& a, bool cache_bf16, cudaStream_t s);
+int score_f32_splits(int tiles, int heads, int most_keys, int sms);
+void launch_score_f32(const ScoreF32Args& a, cudaStream_t s);
 
 // How the matrix-product kernels cap scores: not, by the fast form (bf16 outputs, caps up to
 // kScoreFastCap; q is then scaled by 1 / (8 cap)) or by tanhf (q scaled by log2(e) / 8, as
