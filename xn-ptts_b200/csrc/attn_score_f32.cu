@@ -214,8 +214,8 @@ __global__ void __launch_bounds__(256) score_f32_merge_kernel(ScoreF32Args a) {
 }  // namespace
 
 int score_f32_splits(int tiles, int heads, int most_keys, int sms) {
-    // Two CTAs an SM, each with two key tiles or more.
-    const long long want = 2LL * sms / ((long long)tiles * heads), most = most_keys / (2 * TK);
+    // Four CTAs an SM (their shared memory and registers fit), each with two key tiles or more.
+    const long long ctas = (long long)tiles * heads, want = (4LL * sms + ctas - 1) / ctas, most = most_keys / (2 * TK);
     return (int)(want < most ? (want > 1 ? want : 1) : (most > 1 ? most : 1));
 }
 
