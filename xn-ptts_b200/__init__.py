@@ -160,9 +160,10 @@ def lib() -> ctypes.CDLL:
         L.ptts_b200_kv_copy_stream.argtypes = [P, I, P, I, P]
         L.ptts_b200_kv_check.argtypes = [P]
         L.ptts_b200_attend.argtypes = [P, I, P, P, P, I, I, IP, IP, I, F, P, I, P]
-        L.ptts_b200_attend_scored.argtypes = [P, I, P, P, P, I, I, IP, IP, I, F, ctypes.POINTER(Scores), P, I, P]
-        L.ptts_b200_attend_tree.argtypes = [P, I, P, P, P, I, I, IP, IP, I, P, F, ctypes.POINTER(Scores), P, I, P]
-        L.ptts_b200_kv_accept.argtypes = [P, IP, IP, IP, I, P]
+        # Lists go in as addresses: a ctypes pointer object costs a microsecond.
+        L.ptts_b200_attend_scored.argtypes = [P, I, P, P, P, I, I, P, P, I, F, ctypes.POINTER(Scores), P, I, P]
+        L.ptts_b200_attend_tree.argtypes = [P, I, P, P, P, I, I, P, P, I, P, F, ctypes.POINTER(Scores), P, I, P]
+        L.ptts_b200_kv_accept.argtypes = [P, P, P, P, I, P]
         L.ptts_b200_linear_i8.argtypes = [I, P, P, P, I, I, I, P, P]
         L.ptts_b200_model_create.argtypes = [I, ctypes.POINTER(Config), ctypes.POINTER(P)]
         L.ptts_b200_model_destroy.argtypes = [P]
@@ -226,14 +227,14 @@ def _stream(stream=None) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def _stream_of(device: int, stream=None) -> ctypes.c_void_p:
+def _stream_of(device: int, stream=None) -> int:
     """The CUDA stream handle for a call on `device`, which need not be the current one: `stream`'s,
     else torch's current stream there."""
     import torch
     if stream is not None:
-        return ctypes.c_void_p(stream.cuda_stream)
+        return stream.cuda_stream
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return ctypes.c_void_p(raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream)
+    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 def _dptr(t) -> ctypes.c_void_p:
@@ -400,14 +401,14 @@ class KvState:
         the stream grows by their number (ptts_b200_kv_accept)."""
         if len(nodes) != len(streams):
             raise PttsError(ERR_ARG, "one path per stream")
-        st, counts = _i32(streams), np.fromiter(map(len, nodes), np.int32, len(nodes))
+        st, counts = _vec32(streams), np.fromiter(map(len, nodes), np.int32, len(nodes))
         try:  # node indexes are below 64: lists of them flatten fastest as bytes
             if not set(map(type, nodes)) <= {list, tuple}:
                 raise ValueError
             flat = np.frombuffer(b"".join(map(bytes, nodes)), np.uint8).astype(np.int32)
         except (ValueError, TypeError):  # other sequences, or indexes that the library will refuse
             flat = _i32([x for path in nodes for x in path])
-        _check(lib().ptts_b200_kv_accept(self._h, _ip(st), _ip(counts), _ip(flat), len(st),
+        _check(lib().ptts_b200_kv_accept(self._h, st.ctypes.data, counts.ctypes.data, flat.ctypes.data, st.size,
                                          _stream_of(self.device, stream)))
 
     def check(self):
@@ -444,51 +445,65 @@ def _rule_tensor(kv: KvState, t, name: str, dtype, n: int):
     """The device pointer of a rule's vector (None: NULL), checked."""
     if t is None:
         return None
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != (n,) or not t.is_contiguous():
         raise PttsError(ERR_ARG, f"{name} must be a contiguous vector of {n} {dtype}")
-    if t.device.type != "cuda" or t.device.index != kv.device:
+    if t.get_device() != kv.device:
         raise PttsError(ERR_ARG, f"{name} must be on cuda:{kv.device}, where the cache is")
     return t.data_ptr()
 
 
+def _vec32(a) -> np.ndarray:
+    """_i32, without a copy or a conversion of what is an int32 vector already."""
+    return a if type(a) is np.ndarray and a.dtype == np.int32 and a.flags.c_contiguous else _i32(a)
+
+
 def _attend_rules(kv: KvState, layer, q, k, v, streams, rows, parents, tree, softcap, slopes, first, last, max_period,
                   out_dtype, out, stream):
+    # A single token's call is bound by the host: each line here is a good part of a microsecond.
     import torch
-    if q.dtype != k.dtype or q.dtype != v.dtype:
-        raise PttsError(ERR_ARG, "q, k and v must share a dtype")
-    code = _dtype_code(q)
-    s, r = _i32(streams), _i32(rows)
+    s, r = _vec32(streams), _vec32(rows)
     if s.ndim != 1 or s.shape != r.shape:
         raise PttsError(ERR_ARG, "one row count per stream")
-    n, H, D = int(r.sum()), kv.num_heads, kv.head_dim
-    if q.dim() != 3 or k.dim() != 3 or tuple(q.shape) != (n, H, D) or k.shape != v.shape or k.shape[0] != n or k.shape[2] != D:
+    n, H, D, device = r.item() if r.size == 1 else int(r.sum()), kv.num_heads, kv.head_dim, kv.device
+    code, ks = _dtype_code(q), k.shape
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise PttsError(ERR_ARG, "q, k and v must share a dtype")
+    if q.shape != (n, H, D) or ks != v.shape or len(ks) != 3 or ks[0] != n or ks[2] != D:
         raise PttsError(ERR_ARG, f"expected q [{n}, {H}, {D}] and k, v [{n}, KVH, {D}]")
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if not t.is_contiguous():
-            raise PttsError(ERR_ARG, f"{name} must be contiguous")
-        if t.device.type != "cuda" or t.device.index != kv.device:
-            raise PttsError(ERR_ARG, f"{name} must be on cuda:{kv.device}, where the cache is")
+    if not (q.is_contiguous() and k.is_contiguous() and v.is_contiguous()):
+        raise PttsError(ERR_ARG, "q, k and v must be contiguous")
+    if q.get_device() != device or k.get_device() != device or v.get_device() != device:
+        raise PttsError(ERR_ARG, f"q, k and v must be on cuda:{device}, where the cache is")
     if out is None:
         if out_dtype not in _DTYPES:
             raise PttsError(ERR_ARG, f"unknown out_dtype {out_dtype}")
-        dtype = torch.bfloat16 if _DTYPES[out_dtype] == BF16 else torch.float32
+        out_code = _DTYPES[out_dtype]
         if stream is None:
-            out = torch.empty((n, H * D), dtype=dtype, device=q.device)
+            out = q.new_empty((n, H * D), dtype=torch.bfloat16 if out_code == BF16 else torch.float32)
         else:  # memory of the stream that writes it
             with torch.cuda.stream(stream):
-                out = torch.empty((n, H * D), dtype=dtype, device=q.device)
-    elif tuple(out.shape) != (n, H * D) or not out.is_contiguous() or out.device != q.device:
-        raise PttsError(ERR_ARG, f"out must be a contiguous [{n}, {H * D}] on cuda:{kv.device}")
-    rules = Scores(softcap, _rule_tensor(kv, slopes, "slopes", torch.float32, H),
-                   _rule_tensor(kv, first, "first", torch.int32, n), _rule_tensor(kv, last, "last", torch.int32, n))
-    args = (kv.handle, layer, q.data_ptr(), k.data_ptr(), v.data_ptr(), code, int(k.shape[1]), _ip(s), _ip(r), len(s))
-    tail = (max_period, ctypes.byref(rules), out.data_ptr(), _dtype_code(out), _stream_of(kv.device, stream))
+                out = q.new_empty((n, H * D), dtype=torch.bfloat16 if out_code == BF16 else torch.float32)
+    else:
+        out_code = _dtype_code(out)
+        if out.shape != (n, H * D) or not out.is_contiguous() or out.get_device() != device:
+            raise PttsError(ERR_ARG, f"out must be a contiguous [{n}, {H * D}] on cuda:{device}")
+    rules = None
+    if softcap or slopes is not None or first is not None or last is not None:
+        rules = ctypes.byref(Scores(softcap, _rule_tensor(kv, slopes, "slopes", torch.float32, H),
+                                    _rule_tensor(kv, first, "first", torch.int32, n),
+                                    _rule_tensor(kv, last, "last", torch.int32, n)))
     if tree:
         if parents is None:
             raise PttsError(ERR_ARG, "parents are missing")
-        _check(lib().ptts_b200_attend_tree(*args, _rule_tensor(kv, parents, "parents", torch.int32, n), *tail))
+        rc = lib().ptts_b200_attend_tree(kv._h, layer, q.data_ptr(), k.data_ptr(), v.data_ptr(), code, ks[1], s.ctypes.data,
+                                         r.ctypes.data, s.size, _rule_tensor(kv, parents, "parents", torch.int32, n),
+                                         max_period, rules, out.data_ptr(), out_code, _stream_of(device, stream))
     else:
-        _check(lib().ptts_b200_attend_scored(*args, *tail))
+        rc = lib().ptts_b200_attend_scored(kv._h, layer, q.data_ptr(), k.data_ptr(), v.data_ptr(), code, ks[1], s.ctypes.data,
+                                           r.ctypes.data, s.size, max_period, rules, out.data_ptr(), out_code,
+                                           _stream_of(device, stream))
+    if rc != OK:
+        _check(rc)
     return out
 
 
