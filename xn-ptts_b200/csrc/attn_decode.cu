@@ -30,8 +30,9 @@
 // DEV_ERR_TIMEOUT.
 //
 // With score rules (SCORED): the same split and ring over each row's visible span, its scores capped
-// and biased in f32 between the dot product and the running maximum (see score.h). The rules cost
-// issue slots the copies leave idle: see the rates below the kernel
+// and biased in f32 between the dot product and the running maximum (see score.h). One lane computes a
+// row's rules and exponential, so capped scores keep the copies as the bound: 256 ragged streams of 64-2048
+// keys, one token each, 6.06 TB/s for a whole call (with every lane computing them, 5.1).
 #include "common.cuh"
 #include "kernels.h"
 #include "score.cuh"
@@ -395,6 +396,47 @@ __global__ void __launch_bounds__(kThreads, 1) decode_attn_kernel(DecodeArgs a) 
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[st]);
         }
+        if constexpr (SCORED) {
+            // Lane j of a group takes over the group's row j: the rules, the exponential and the running
+            // maximum once per row (in the loop below every lane of a group has all of them).
+            float u = 0.f;
+#pragma unroll
+            for (int i = 0; i < RPL; ++i) {
+                const int r = 4 * i + g;
+                Raw<T> rk;
+                load_raw(ks + (r < n ? r : n - 1) * RB, j, rk);
+                float k[8], d = 0.f;
+                widen(rk, k);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) d = fmaf(q[e], k[e], d);
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+                u = j == i ? d : u;
+            }
+            const int mine = 4 * j + g;
+            u = score_exact(u, a.cap, inv_cap, slope, hd.at - p - mine);
+            if (j >= RPL || mine >= n) u = -INFINITY;
+            float mn = u;
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+            mn = fmaxf(m, mn);
+            const float corr = fast_exp2(m - mn), e = fast_exp2(u - mn);
+            l = fmaf(l, corr, e);  // this lane's rows
+            m = mn;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] *= corr;
+#pragma unroll
+            for (int i = 0; i < RPL; ++i) {
+                const int r = 4 * i + g;
+                Raw<T> rv;
+                load_raw(vs + (r < n ? r : n - 1) * RB, j, rv);
+                float v[8];
+                widen(rv, v);
+                const float w = __shfl_sync(0xffffffffu, e, (lane & 24) | i);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) acc[x] = fmaf(w, v[x], acc[x]);
+            }
+        } else {
 #pragma unroll
         for (int i = 0; i < RPL; i += 2) {
             if (4 * i >= n) break;
@@ -421,10 +463,6 @@ __global__ void __launch_bounds__(kThreads, 1) decode_attn_kernel(DecodeArgs a) 
                 d0 += __shfl_xor_sync(0xffffffffu, d0, o);
                 d1 += __shfl_xor_sync(0xffffffffu, d1, o);
             }
-            if constexpr (SCORED) {
-                d0 = score_exact(d0, a.cap, inv_cap, slope, hd.at - p - r0);
-                d1 = score_exact(d1, a.cap, inv_cap, slope, hd.at - p - r1);
-            }
             if (r0 >= n) d0 = -INFINITY;
             if (r1 >= n) d1 = -INFINITY;
             if (vis) {
@@ -447,6 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_attn_kernel(DecodeArgs a) 
             for (int e = 0; e < 8; ++e) acc[e] = fmaf(e1, v1[e], fmaf(e0, v0[e], acc[e] * corr));
             m = mn;
         }
+        }
         if constexpr (!R::kStaged) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[st]);
@@ -455,6 +494,10 @@ __global__ void __launch_bounds__(kThreads, 1) decode_attn_kernel(DecodeArgs a) 
         // The end of this CTA's piece of stream b: merge the four row groups (lanes j, j+8,
         // j+16, j+24 hold the same dims).
         float mm = m, ll = l, aa[8];
+        if constexpr (SCORED) {
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) aa[i] = acc[i];
 #pragma unroll
