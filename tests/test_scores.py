@@ -274,16 +274,21 @@ def test_scored_heads_and_types(ptts, cuda, shape, heads, kv_heads, dtype, in_dt
 
 @pytest.mark.gpu
 def test_without_rules_it_is_attend(ptts, cuda):
-    """No rules: the same rows in the cache as attend's, bit for bit, and its outputs within both bounds."""
+    """No rules: attend's values in the cache bit for bit, its keys but for the last step of a rotation (sine
+    and cosine rounded once here, sincosf's there: 2 f32 steps, at most one bf16 step, 2^-7), and its
+    outputs within the same bound."""
     import torch
     for shape in ("tokens", "mixed", "prompt_keys"):
         a, b = (Batch(ptts, cuda, *SHAPES[shape], seed=3) for _ in range(2))
         out, want, bound = call(a, {})
         ref = ptts.attend(b.kv, 0, b.q, b.k, b.v, b.streams, b.rows)
         compare(out, want, bound)
-        compare(ref, want, bound)
-        for x, y in zip(a.kv.tensors(0), b.kv.tensors(0)):
-            assert torch.equal(torch.nan_to_num(x), torch.nan_to_num(y))
+        compare(ref, *b.want(half_p=PAIR_HALF))
+        (ka, va, la), (kb, vb, lb) = a.kv.tensors(0), b.kv.tensors(0)
+        assert torch.equal(torch.nan_to_num(va), torch.nan_to_num(vb)) and torch.equal(la, lb)
+        x, y = torch.nan_to_num(ka).double(), torch.nan_to_num(kb).double()
+        assert ((x - y).abs() <= 2.0 ** -7 * x.abs() + 2.0 ** -20).all()
+        a.check_rows(), b.check_rows()
 
 
 @pytest.mark.gpu

@@ -180,8 +180,8 @@ struct ptts_b200_kv {
     std::vector<int32_t> h_window;
     // scratch of the attention op
     DevBuf seq_stream, row_offsets, row_stream, row_pos, prefix, part, q_rot, counters;
-    // scratch of the scored and tree attention: the rows' plan, their lineages, the work units
-    DevBuf score_rows, lineage, units;
+    // scratch of the scored and tree attention, one allocation for a call's lists, plan, q and records
+    DevBuf score;
     Staging staging;
     // What seq_stream holds after the last upload_seq, and on which CUDA stream it was copied: a
     // decode loop that attends and advances the same streams step after step copies the list
@@ -640,10 +640,40 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
     std::vector<int32_t> packed(streams_host, streams_host + n_seq);
     packed.insert(packed.end(), offsets.begin(), offsets.end());
     const size_t blocks_at = append_tiles(packed, blocks);
-    const int32_t* d = kv->upload_seq(packed, s);
+    const bool inlined = packed.size() <= (size_t)kScoreInline;
+    const int n_units = few ? n_seq : tokens ? n_rows : 0;
+    long long keys = 0;
+    int most_keys = 0;
+    for (int i = 0; i < n_seq; ++i) {
+        keys += kv->h_len[streams_host[i]] + rows_host[i];
+        most_keys = std::max(most_keys, kv->h_len[streams_host[i]] + rows_host[i]);
+    }
+    const int splits = !tokens && !cache_bf16 ? score_f32_splits((int)blocks.size(), kv->heads, most_keys, grid) : 1;
+    const size_t part_floats = tokens ? decode_part_floats(n_rows, grid) * kv->groups()
+                               : few  ? score_rows_part_floats(kv->heads, grid, keys, most)
+                                      : splits > 1 ? (size_t)kPartStride * splits * kv->heads * n_rows : 0;
+    // The scratch, cut into 256-byte aligned parts.
+    size_t bytes = 0;
+    auto part = [&](size_t n) {
+        const size_t at = bytes;
+        bytes += (n + 255) / 256 * 256;
+        return at;
+    };
+    const size_t at_list = part(inlined ? sizeof(int32_t) * packed.size() : 0), at_q = part((size_t)n_rows * hd * sizeof(float)),
+                 at_rows = part(sizeof(int32_t) * (tree ? 6 : 4) * (size_t)n_rows),
+                 at_lineage = part(tree ? sizeof(unsigned long long) * (size_t)n_rows : 0),
+                 at_units = part(n_units ? sizeof(int32_t) * (2 * (size_t)n_units + 1 + grid) : 0),
+                 at_part = part(sizeof(float) * part_floats);
+    char* ws = static_cast<char*>(kv->score.need(bytes));
+    // A short list rides in the plan's parameters, and the plan leaves it in the scratch for the kernels
+    // after it.
+    ScoreInline in;
+    if (inlined) std::copy(packed.begin(), packed.end(), in.list);
+    const int32_t* d = inlined ? reinterpret_cast<const int32_t*>(ws + at_list) : kv->upload_seq(packed, s);
+    float* records = reinterpret_cast<float*>(ws + at_part);
     ScorePlanArgs p{};
-    p.seq_stream = d;
-    p.row_offsets = d + n_seq;
+    p.list = const_cast<int32_t*>(d);
+    p.list_ints = (int)packed.size();
     p.n_seq = n_seq;
     p.n_rows = n_rows;
     p.lengths = kv->len.as<int32_t>();
@@ -655,14 +685,14 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
     p.q = q;
     p.k = k;
     p.v = v;
-    p.q_out = static_cast<float*>(kv->q_rot.need((size_t)n_rows * hd * sizeof(float)));
+    p.q_out = reinterpret_cast<float*>(ws + at_q);
     p.k_cache = kv->k_layer(layer);
     p.v_cache = kv->v_layer(layer);
     p.heads = kv->heads;
     p.kv_heads = num_kv_heads;
     p.rotate = max_period != 0.0f;
     if (p.rotate) rope_inv_freq(kv->head_dim, max_period, p.inv_freq);
-    int32_t* rows = static_cast<int32_t*>(kv->score_rows.need(sizeof(int32_t) * (tree ? 6 : 4) * (size_t)n_rows));
+    int32_t* rows = reinterpret_cast<int32_t*>(ws + at_rows);
     p.rows.stream = rows;
     p.rows.pos = rows + n_rows;
     p.rows.lo = rows + 2 * (size_t)n_rows;
@@ -670,24 +700,25 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
     if (tree) {
         p.rows.base = rows + 4 * (size_t)n_rows;
         p.rows.row0 = rows + 5 * (size_t)n_rows;
-        p.rows.lineage = static_cast<unsigned long long*>(kv->lineage.need(sizeof(unsigned long long) * n_rows));
+        p.rows.lineage = reinterpret_cast<unsigned long long*>(ws + at_lineage);
     }
     p.err = kv->err.as<uint32_t>();
     if (tokens || few) {
-        p.n_units = few ? (int)blocks.size() : n_rows;
-        p.blocks = few ? reinterpret_cast<const int2*>(d + blocks_at) : nullptr;
+        p.n_units = n_units;
+        p.blocks_at = few ? (int)blocks_at : -1;
         p.grid = grid;
-        p.prefix = static_cast<int32_t*>(kv->units.need(sizeof(int32_t) * (2 * (size_t)p.n_units + 1 + grid)));
-        p.unit_lo = p.prefix + p.n_units + 1;
-        p.cta_first = p.unit_lo + p.n_units;
+        p.prefix = reinterpret_cast<int32_t*>(ws + at_units);
+        p.unit_lo = p.prefix + n_units + 1;
+        p.cta_first = p.unit_lo + n_units;
     }
     if (few || prompt) {  // two bf16 planes in the f32 buffer
         p.q_hi = reinterpret_cast<__nv_bfloat16*>(p.q_out);
         p.q_lo = p.q_hi + (size_t)n_rows * hd;
         p.q_scale = score_q_scale(sc.softcap, !out_bf16);
     }
-    launch_score_plan(p, in_dtype == PTTS_B200_BF16, cache_bf16, s);
+    launch_score_plan(p, inlined ? &in : nullptr, in_dtype == PTTS_B200_BF16, cache_bf16, s);
     check_launch();
+    const int2* d_blocks = reinterpret_cast<const int2*>(d + blocks_at);
     if (tokens) {
         const size_t n_part = decode_part_floats(n_rows, grid), n_cnt = decode_counter_ints(n_rows);
         const size_t out_elem = out_dtype == PTTS_B200_BF16 ? 2 : 4;
@@ -708,7 +739,7 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
             a.out = static_cast<char*>(out) + col * out_elem;
             a.out_mode = out_dtype == PTTS_B200_BF16 ? kOutBf16 : kOutF32;
             a.ld = (int)hd;
-            a.part = static_cast<float*>(kv->part.need(sizeof(float) * n_part * kv->groups())) + n_part * g;
+            a.part = records + n_part * g;
             a.counters = static_cast<int*>(kv->counters.need_zeroed(sizeof(int) * n_cnt * kv->groups())) + n_cnt * g;
             a.B = n_rows;
             a.capacity = kv->capacity;
@@ -735,14 +766,14 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
         a.rows = p.rows;
         a.rule.cap = sc.softcap;
         a.rule.slopes = sc.slopes;
-        a.blocks = p.blocks;
+        a.blocks = d_blocks;
         a.n_units = p.n_units;
         a.prefix = p.prefix;
         a.unit_lo = p.unit_lo;
         a.cta_first = p.cta_first;
         a.n_rows = n_rows;
         a.most_rows = most;
-        a.part = static_cast<float*>(kv->part.need(sizeof(float) * score_rows_part_floats(kv->heads, grid)));
+        a.part = records;
         a.err = p.err;
         require(launch_score_rows(a, grid, s), PTTS_B200_ERR_CUDA,
                 "could not describe the cache's tensors (cuTensorMapEncodeTiled)");
@@ -765,7 +796,7 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
         a.rows = p.rows;
         a.rule.cap = sc.softcap;
         a.rule.slopes = sc.slopes;
-        a.tiles = reinterpret_cast<const int2*>(d + blocks_at);
+        a.tiles = d_blocks;
         a.n_tiles = (int)blocks.size();
         // Several heads a CTA share its start and fetch ahead across heads, as long as every SM's two
         // CTAs still get two or more to even out.
@@ -790,13 +821,10 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
     a.rows = p.rows;
     a.rule.cap = sc.softcap;
     a.rule.slopes = sc.slopes;
-    a.tiles = reinterpret_cast<const int2*>(d + blocks_at);
+    a.tiles = d_blocks;
     a.n_tiles = (int)blocks.size();
-    int most_keys = 0;
-    for (int i = 0; i < n_seq; ++i) most_keys = std::max(most_keys, kv->h_len[streams_host[i]] + rows_host[i]);
-    a.splits = score_f32_splits(a.n_tiles, kv->heads, most_keys, grid);
-    if (a.splits > 1)
-        a.part = static_cast<float*>(kv->part.need(sizeof(float) * kPartStride * a.splits * kv->heads * (size_t)n_rows));
+    a.splits = splits;
+    a.part = records;
     launch_score_f32(a, s);
     check_launch();
 }

@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
                 const bool bad = R->bad != 0;
                 const long long at = (long long)w.row0 * a.ld + head * kHeadDim + key;
                 // Record 2 c of a piece that began before this CTA's range, 2 c + 1 of one that begins in it.
-                float* rec = a.part + ((long long)(2 * c + (w.begins ? 1 : 0)) * a.heads + head) * NR * kPartStride;
+                float* rec = a.part + ((long long)(2 * c + (w.begins ? 1 : 0)) * a.heads + head) * a.most_rows * kPartStride;
                 // Rolled: code that runs once a piece costs more to fetch than to run.
 #pragma unroll 1
                 for (int g = 0; g < groups; ++g) {
@@ -592,7 +592,7 @@ const int rows = w.nrows - 16 * g;  // of these 16
 // Joins the pieces of the blocks that CTAs' ranges cut: one warp per row and head, lane = 2 dims.
 // Every warp reads the pieces' maxima and sums lane by lane and then all records at once.
 template <bool P2>
-__global__ void __launch_bounds__(256) score_rows_merge_kernel(ScoreRowsArgs a, int grid, int rows_max) {
+__global__ void __launch_bounds__(256) score_rows_merge_kernel(ScoreRowsArgs a, int grid) {
     grid_dep_wait();
     grid_dep_launch();
     const long long total = a.prefix[a.n_units];
@@ -604,7 +604,7 @@ __global__ void __launch_bounds__(256) score_rows_merge_kernel(ScoreRowsArgs a, 
     const int r = blockIdx.z * 8 + (threadIdx.x >> 5);
     if (r >= rows.y) return;
     auto rec = [&](int c) {
-        return a.part + (((long long)(2 * c + (c == c0 ? 1 : 0)) * a.heads + head) * rows_max + r) * kPartStride;
+        return a.part + (((long long)(2 * c + (c == c0 ? 1 : 0)) * a.heads + head) * a.most_rows + r) * kPartStride;
     };
     float mx = kScoreLow;
     for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, rec(c)[64]);
@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(256) score_rows_merge_kernel(ScoreRowsArgs a, 
 template <bool P2>
 void merge(const ScoreRowsArgs& a, int grid, cudaStream_t s) {
     if (grid > 1)
-        launch_k(score_rows_merge_kernel<P2>, dim3(a.n_units, a.heads, (a.most_rows + 7) / 8), dim3(256), 0, s, a, grid, NR);
+        launch_k(score_rows_merge_kernel<P2>, dim3(a.n_units, a.heads, (a.most_rows + 7) / 8), dim3(256), 0, s, a, grid);
 }
 
 template <int HC, int CAP, bool BOUNDED, bool P2>
@@ -657,7 +657,10 @@ int score_rows_grid(bool out_bf16, int heads, int sms) {
     return sms / slabs > 1 ? sms / slabs : 1;
 }
 
-size_t score_rows_part_floats(int heads, int grid) { return (size_t)2 * grid * heads * NR * kPartStride; }
+size_t score_rows_part_floats(int heads, int grid, long long keys, int most_rows) {
+    const long long ctas = (keys + kMinKeysPerCta - 1) / kMinKeysPerCta;  // ctas_in_use, at most
+    return (size_t)2 * (ctas < grid ? ctas : grid) * heads * most_rows * kPartStride;
+}
 
 bool launch_score_rows(const ScoreRowsArgs& a, int grid, cudaStream_t s) {
     CUtensorMap m[4];

@@ -32,9 +32,11 @@ struct ScoreRule {
 };
 
 struct ScorePlanArgs {
-    // What the host sends: streams [n_seq], row offsets [n_seq + 1].
-    const int32_t* seq_stream;
-    const int32_t* row_offsets;
+    // What the host sends: streams [n_seq], row offsets [n_seq + 1], and from blocks_at on the work
+    // units or tiles as (first row, rows). An inline list is written to `list` (for the kernels after the
+    // plan); else it is there.
+    int32_t* list;
+    int list_ints;
     int n_seq, n_rows;
     const int32_t* lengths;   // [num_streams]
     int num_streams, capacity;
@@ -57,7 +59,7 @@ struct ScorePlanArgs {
     ScoreRows rows;
     // Split kernels: the work units (single rows, or blocks of consecutive rows of one sequence:
     // (first row, rows)), their key counts laid end to end, and the unit each CTA starts in.
-    const int2* blocks = nullptr;  // [n_units]; nullptr: unit u is row u
+    int blocks_at = -1;            // where the blocks are in the list; -1: unit u is row u
     int n_units = 0;               // 0: no units
     int32_t* prefix = nullptr;     // [n_units + 1]
     int32_t* unit_lo = nullptr;    // [n_units] first slot any row of the unit sees
@@ -65,8 +67,12 @@ struct ScorePlanArgs {
     int grid = 0;
     uint32_t* err;
 };
+constexpr int kScoreInline = 768;
+struct ScoreInline {  // a short list rides in the launch's parameters
+    int32_t list[kScoreInline];
+};
 // One launch: every row's plan entry, its rotated q, its cache rows; and the units' partition.
-void launch_score_plan(const ScorePlanArgs& a, bool in_bf16, bool cache_bf16, cudaStream_t s);
+void launch_score_plan(const ScorePlanArgs& a, const ScoreInline* list, bool in_bf16, bool cache_bf16, cudaStream_t s);
 
 // Prompts and trees on f32 caches (attn_score_f32.cu): tiles (first row, rows) of up to kScoreF32Rows rows
 // of one sequence; with splits > 1 the tiles' keys are shared out and joined through `part`.
@@ -125,7 +131,8 @@ struct ScoreRowsArgs {
     uint32_t* err;
 };
 int score_rows_grid(bool out_bf16, int heads, int sms);  // CTAs along the keys (the plan's grid)
-size_t score_rows_part_floats(int heads, int grid);
+// For `keys` keys of all blocks (an upper bound) and blocks of up to most_rows rows.
+size_t score_rows_part_floats(int heads, int grid, long long keys, int most_rows);
 bool launch_score_rows(const ScoreRowsArgs& a, int grid, cudaStream_t s);
 
 // Prompts on tcgen05, bf16 caches (attn_score_prompt.cu): tiles (first row, rows) of up to 128

@@ -17,9 +17,8 @@ constexpr int kPlanThreads = 256;
 constexpr int kPlanWarps = kPlanThreads / 32;
 
 // The last sequence whose rows begin at or before row r.
-__device__ __forceinline__ int seq_of(const ScorePlanArgs& a, int r) {
+__device__ __forceinline__ int seq_of(const ScorePlanArgs& a, const int32_t* offsets, int r) {
     if (a.n_seq == a.n_rows) return r;  // single tokens
-    const int32_t* offsets = a.row_offsets;
     int lo = 0, hi = a.n_seq - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -30,12 +29,12 @@ __device__ __forceinline__ int seq_of(const ScorePlanArgs& a, int r) {
 }
 
 // The same by a warp for one row: 31 probes a step.
-__device__ __forceinline__ int seq_of_warp(const ScorePlanArgs& a, int r, int lane) {
+__device__ __forceinline__ int seq_of_warp(const ScorePlanArgs& a, const int32_t* offsets, int r, int lane) {
     if (a.n_seq == a.n_rows) return r;
     int lo = 0, hi = a.n_seq - 1;  // offsets[lo] <= r, offsets[hi + 1] > r
     while (lo < hi) {
         const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step;
-        const int below = __popc(__ballot_sync(0xffffffffu, at <= hi && a.row_offsets[min(at, hi)] <= r));
+        const int below = __popc(__ballot_sync(0xffffffffu, at <= hi && offsets[min(at, hi)] <= r));
         lo += below * step;
         hi = min(hi, lo + step - 1);
     }
@@ -53,21 +52,23 @@ __device__ __forceinline__ void row_span(const ScorePlanArgs& a, int r, int base
 
 // CTA 0: the units' key counts, end to end. Every unit has at least one key, so that a CTA visits
 // it and writes its rows even where they see nothing.
-__device__ void plan_units(const ScorePlanArgs& a) {
+__device__ __forceinline__ void plan_units(const ScorePlanArgs& a, const int32_t* list) {
     __shared__ int warp_tot[kPlanWarps];
     __shared__ int carry;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const bool spans = a.first || a.last;
+    const bool spans = a.first || a.last, blocks = a.blocks_at >= 0;
+    const int32_t *streams = list, *offsets = list + a.n_seq, *units = list + a.blocks_at;
+    auto unit = [&](int u) { return blocks ? make_int2(units[2 * u], units[2 * u + 1]) : make_int2(u, 1); };
     if (tid == 0) {
         carry = 0;
         a.prefix[0] = 0;
     }
     // A block's union of spans: a warp per block, two rows a lane.
-    if (a.blocks && spans) {
+    if (blocks && spans) {
         for (int u = warp; u < a.n_units; u += kPlanWarps) {
-            const int2 b = a.blocks[u];
-            const int sq = seq_of(a, b.x), row0 = a.row_offsets[sq];
-            const int base = a.lengths[a.seq_stream[sq]], rows = a.row_offsets[sq + 1] - row0;
+            const int2 b = unit(u);
+            const int sq = seq_of(a, offsets, b.x), row0 = offsets[sq];
+            const int base = a.lengths[streams[sq]], rows = offsets[sq + 1] - row0;
             int lo = 0x7fffffff, hi = -1;
             for (int i = lane; i < b.y; i += 32) {
                 int x, y;
@@ -90,12 +91,12 @@ __device__ void plan_units(const ScorePlanArgs& a) {
         const int u = at + tid;
         int v = 0;
         if (u < a.n_units) {
-            if (a.blocks && spans) {
+            if (blocks && spans) {
                 v = a.prefix[u + 1];
             } else {
-                const int2 b = a.blocks ? a.blocks[u] : make_int2(u, 1);
-                const int sq = seq_of(a, b.x), row0 = a.row_offsets[sq];
-                const int base = a.lengths[a.seq_stream[sq]], rows = a.row_offsets[sq + 1] - row0;
+                const int2 b = unit(u);
+                const int sq = seq_of(a, offsets, b.x), row0 = offsets[sq];
+                const int base = a.lengths[streams[sq]], rows = offsets[sq + 1] - row0;
                 int lo, hi;
                 row_span(a, b.x + b.y - 1, base, row0, rows, lo, hi);  // without spans the last row sees the most
                 a.unit_lo[u] = lo;
@@ -151,23 +152,22 @@ __device__ __forceinline__ void store_out(__nv_bfloat16* p, const float* x) {
 }
 
 template <typename Tin, typename T>
-__global__ void __launch_bounds__(kPlanThreads) score_plan_kernel(ScorePlanArgs a) {
-    grid_dep_wait();
-    grid_dep_launch();
+__device__ __forceinline__ void plan(const ScorePlanArgs& a, const int32_t* list) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int block = blockIdx.x;
     if (a.n_units > 0) {
         if (block == 0) {
-            plan_units(a);
+            plan_units(a, list);
             return;
         }
         block -= 1;
     }
+    const int32_t* offsets = list + a.n_seq;
     // A warp per row.
     const int r = block * kPlanWarps + warp;
     if (r >= a.n_rows) return;
-    const int sq = seq_of_warp(a, r, lane), row0 = a.row_offsets[sq];
-    const int rows = a.row_offsets[sq + 1] - row0, sid = a.seq_stream[sq];
+    const int sq = seq_of_warp(a, offsets, r, lane), row0 = offsets[sq];
+    const int rows = offsets[sq + 1] - row0, sid = list[sq];
     const bool known = sid >= 0 && sid < a.num_streams;
     const int base = known ? a.lengths[sid] : 0;
     const int node = r - row0, slot = base + node;
@@ -216,8 +216,11 @@ __global__ void __launch_bounds__(kPlanThreads) score_plan_kernel(ScorePlanArgs 
     constexpr int E = 16 / (int)sizeof(Tin), HS = 32 * E / kHeadDim;
     float cs[E / 2], sn[E / 2];
     if (a.rotate) {
-        float s, c;
-        sincosf((float)pos * a.inv_freq[lane], &s, &c);
+        // The f32 angle's sine and cosine in f64, rounded once (attend's are sincosf's: a key in one of
+        // ten thousand ends up a bf16 step apart). Beside the row's memory traffic it does not show.
+        double sd, cd;
+        sincos((double)((float)pos * a.inv_freq[lane]), &sd, &cd);
+        const float s = (float)sd, c = (float)cd;
 #pragma unroll
         for (int i = 0; i < E / 2; ++i) {
             const int pair = lane % (kHeadDim / E) * (E / 2) + i;
@@ -275,14 +278,36 @@ __global__ void __launch_bounds__(kPlanThreads) score_plan_kernel(ScorePlanArgs 
     }
 }
 
+template <typename Tin, typename T>
+__global__ void __launch_bounds__(kPlanThreads) score_plan_kernel(ScorePlanArgs a) {
+    grid_dep_wait();
+    grid_dep_launch();
+    plan<Tin, T>(a, a.list);
+}
+
+template <typename Tin, typename T>
+__global__ void __launch_bounds__(kPlanThreads) score_plan_inline_kernel(ScorePlanArgs a, const __grid_constant__ ScoreInline l) {
+    grid_dep_wait();
+    grid_dep_launch();
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < a.list_ints; i += kPlanThreads) a.list[i] = l.list[i];
+    plan<Tin, T>(a, l.list);
+}
+
+template <typename Tin, typename T>
+void launch_typed(const ScorePlanArgs& a, const ScoreInline* list, cudaStream_t s) {
+    const dim3 grid((a.n_rows + kPlanWarps - 1) / kPlanWarps + (a.n_units > 0 ? 1 : 0)), block(kPlanThreads);
+    if (list) launch_k(score_plan_inline_kernel<Tin, T>, grid, block, 0, s, a, *list);
+    else launch_k(score_plan_kernel<Tin, T>, grid, block, 0, s, a);
+}
+
 }  // namespace
 
-void launch_score_plan(const ScorePlanArgs& a, bool in_bf16, bool cache_bf16, cudaStream_t s) {
-    const dim3 grid((a.n_rows + kPlanWarps - 1) / kPlanWarps + (a.n_units > 0 ? 1 : 0)), block(kPlanThreads);
-    if (in_bf16 && cache_bf16) launch_k(score_plan_kernel<__nv_bfloat16, __nv_bfloat16>, grid, block, 0, s, a);
-    else if (in_bf16) launch_k(score_plan_kernel<__nv_bfloat16, float>, grid, block, 0, s, a);
-    else if (cache_bf16) launch_k(score_plan_kernel<float, __nv_bfloat16>, grid, block, 0, s, a);
-    else launch_k(score_plan_kernel<float, float>, grid, block, 0, s, a);
+void launch_score_plan(const ScorePlanArgs& a, const ScoreInline* list, bool in_bf16, bool cache_bf16, cudaStream_t s) {
+    if (in_bf16 && cache_bf16) launch_typed<__nv_bfloat16, __nv_bfloat16>(a, list, s);
+    else if (in_bf16) launch_typed<__nv_bfloat16, float>(a, list, s);
+    else if (cache_bf16) launch_typed<float, __nv_bfloat16>(a, list, s);
+    else launch_typed<float, float>(a, list, s);
 }
 
 }  // namespace ptts
