@@ -227,8 +227,8 @@ int ptts_b200_attend(ptts_b200_kv* kv, int layer, const void* q, const void* k, 
  * Keys that a row does not see never reach its output, whatever they hold (NaN included).
  * ------------------------------------------------------------------------------------- */
 typedef struct {
-    float softcap;         /* positive, or 0 for none */
-    const float* slopes;   /* [num_heads] f32 (device), or NULL */
+    float softcap;         /* within 1e-30 .. 1e30, or 0 for none */
+    const float* slopes;   /* [num_heads] f32 (device), any sign, or NULL */
     const int32_t* first;  /* [n_rows] (device): the first position a row sees; NULL: 0 */
     const int32_t* last;   /* [n_rows] (device): the last position a row sees; NULL: its own */
 } ptts_b200_scores;

@@ -153,7 +153,7 @@ class Batch:
                 size = size + softcap
             if slopes is not None:
                 bias = slopes.double()[:, None, None] * (pos[:, None] - where[None]).abs().double()[None]
-                u, size = u - bias, size + bias
+                u, size = u - bias, size + bias.abs()
             u = u.masked_fill(~seen[None], -math.inf)
             w = torch.exp(u - u.amax(-1, keepdim=True).clamp(min=-1e300))
             w = w / w.sum(-1, keepdim=True).clamp(min=1e-300)
@@ -211,6 +211,8 @@ SHAPES = {  # name: (cached, rows)
     "prompt_keys": ([0, 130, 1], [65, 300, 127]),
     "prompt_long": ([100], [1100]),
     "rows_over_long_cache": ([5000], [70]),
+    "beside_a_prompt": ([6000, 3000, 0], [1, 40, 200]),
+    "long_list": ([(i * 29) % 90 for i in range(400)], [1 + i % 2 for i in range(400)]),
 }
 RULES = {
     "plain": {},
@@ -219,13 +221,16 @@ RULES = {
     "big_cap": {"softcap": 3e4},
     "bias": {"slopes": True, "max_period": 0.0},
     "cap_bias": {"softcap": 50.0, "slopes": True},
+    "cap_rising_bias": {"softcap": 30.0, "slopes": -0.25},
+    "rising_bias": {"slopes": -1.0},
 }
 
 
 def call(b, rule, mask="causal", out_dtype="f32", layer=0, **kw):
     first, last = b.spans(mask)
     args = dict(rule)
-    slopes = b.slopes if args.pop("slopes", False) else None
+    times = float(args.pop("slopes", 0.0))
+    slopes = b.slopes * times if times else None
     out = b.ptts.attend_scored(b.kv, layer, b.q, b.k, b.v, b.streams, b.rows, first=b.dev(first), last=b.dev(last),
                                slopes=slopes, out_dtype=out_dtype, **args, **kw)
     half_out, half_p = b.halves(out_dtype)
@@ -247,8 +252,10 @@ def test_scored_rules_and_lengths(ptts, cuda, shape, rule, dtype, out_dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("mask", ["prefix", "documents", "window", "wild", "extremes"])
-@pytest.mark.parametrize("shape", ["tokens", "mixed", "short_rows_long_cache", "prompt_tiles", "prompt_keys", "prompt_long"])
-@pytest.mark.parametrize("dtype,rule", [("bf16", "plain"), ("bf16", "cap_bias"), ("f32", "cap_bias")])
+@pytest.mark.parametrize("shape", ["tokens", "mixed", "short_rows_long_cache", "prompt_tiles", "prompt_keys", "prompt_long",
+                                   "beside_a_prompt"])
+@pytest.mark.parametrize("dtype,rule", [("bf16", "plain"), ("bf16", "cap"), ("bf16", "bias"), ("bf16", "cap_bias"),
+                                        ("bf16", "cap_rising_bias"), ("f32", "cap_bias")])
 def test_scored_spans(ptts, cuda, shape, mask, dtype, rule):
     b = Batch(ptts, cuda, *SHAPES[shape], dtype=dtype, seed=len(shape) * 7 + len(mask))
     out, want, bound = call(b, RULES[rule], mask, out_dtype=dtype)
@@ -262,7 +269,7 @@ def test_scored_spans(ptts, cuda, shape, mask, dtype, rule):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("heads,kv_heads", [(8, 1), (8, 2), (16, 16), (16, 4), (24, 8)])
-@pytest.mark.parametrize("shape", ["tokens", "mixed", "prompt_keys"])
+@pytest.mark.parametrize("shape", ["tokens", "mixed", "prompt_keys", "beside_a_prompt"])
 @pytest.mark.parametrize("dtype,in_dtype", [("bf16", "f32"), ("f32", "bf16"), ("bf16", "bf16")])
 def test_scored_heads_and_types(ptts, cuda, shape, heads, kv_heads, dtype, in_dtype):
     b = Batch(ptts, cuda, *SHAPES[shape], heads=heads, kv_heads=kv_heads, dtype=dtype, in_dtype=in_dtype, seed=heads)
@@ -363,19 +370,20 @@ TREES = {
     "empty_cache": ([0, 0], [64, 7]),
     "batch": ([3, 64, 200, 31, 1000], [16, 17, 64, 1, 33]),
     "long": ([6000, 50], [48, 20]),
-    "many": ([(i * 53) % 300 for i in range(160)], [1 + (i * 7) % 64 for i in range(160)]),
+    "many": ([(i * 53) % 300 for i in range(260)], [1 + (i * 7) % 64 for i in range(260)]),
 }
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rule", ["plain", "cap", "bias", "cap_bias"])
+@pytest.mark.parametrize("rule", ["plain", "cap", "bias", "cap_bias", "cap_rising_bias"])
 @pytest.mark.parametrize("shape", list(TREES))
 @pytest.mark.parametrize("dtype,out_dtype", [("bf16", "bf16"), ("bf16", "f32"), ("f32", "f32")])
 @pytest.mark.parametrize("windowed", [False, True])
 def test_tree(ptts, cuda, shape, rule, dtype, out_dtype, windowed):
     b = Batch(ptts, cuda, *TREES[shape], dtype=dtype, seed=len(shape), tree=True)
     args = dict(RULES[rule])
-    slopes = b.slopes if args.pop("slopes", False) else None
+    times = float(args.pop("slopes", 0.0))
+    slopes = b.slopes * times if times else None
     first = None
     if windowed:  # a window of w positions before each node, from none of the cache to all of it
         w = np.repeat([1 + (7 * i) % (int(L) + 9) for i, L in enumerate(b.cached)], b.rows)
@@ -585,7 +593,7 @@ def test_refusals_change_nothing(ptts, cuda):
     refused(ptts.ERR_ARG, scored, rows=[3, 1, 0])
     refused(ptts.ERR_UNSUPPORTED, scored, streams=[st[0], st[1], others[0]])
     refused(ptts.ERR_UNSUPPORTED, scored, streams=[st[0], st[1], others[1]])
-    for cap in (-1.0, float("nan"), float("inf")):
+    for cap in (-1.0, 1e-38, 1e38, float("nan"), float("inf")):
         refused(ptts.ERR_ARG, scored, softcap=cap)
     for period in (1.0, -3.0, float("nan"), float("inf")):
         refused(ptts.ERR_ARG, scored, max_period=period)

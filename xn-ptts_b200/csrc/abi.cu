@@ -579,6 +579,30 @@ void refuse_capture(cudaStream_t s, const char* what) {
         fail(PTTS_B200_ERR_STATE, std::string(what) + " plans from the host's lengths: it cannot be captured in a CUDA graph");
 }
 
+// Which sequences of a call on a bf16 cache run on the rows kernel (blocks of 64 rows split over the keys)
+// rather than in the prompt kernel's tiles of 128 rows. Trees: all. Others by estimated times (us on one
+// B200, 8 heads, measured over 1-64 sequences of 16-512 rows on 0-30000 keys): a tile takes 0.0113 a key
+// however few its rows, and the GPU 0.000305 a tile and key once it is full; the rows kernel takes 0.0005 a
+// block and key, and 14 more to start and join. So a sequence whose tile alone would outlast the whole
+// call's tiles by that goes there (one of 65 rows on 8000 keys: 38 against 102; single tokens beside a
+// prompt), unless all that went there would take longer than its longest tile.
+std::vector<char> few_row_sequences(const ptts_b200_kv* kv, const int32_t* streams, const int32_t* rows, int n_seq,
+                                    bool tree) {
+    std::vector<char> few(n_seq, tree);
+    if (tree) return few;
+    const double per_tile = 0.0113, full = 0.000305 * kv->groups(), per_block = 0.0005 * kv->groups(), start = 14.0;
+    double all = 0.0, blocks = start, longest = 0.0;
+    auto keys = [&](int i) { return (double)kv->h_len[streams[i]] + rows[i]; };
+    for (int i = 0; i < n_seq; ++i) all += full * ((rows[i] + 127) / 128) * keys(i);
+    for (int i = 0; i < n_seq; ++i)
+        if ((few[i] = per_tile * keys(i) > all + start)) {
+            blocks += per_block * ((rows[i] + kTreeNodes - 1) / kTreeNodes) * keys(i);
+            longest = std::max(longest, per_tile * keys(i));
+        }
+    if (blocks > longest) few.assign(n_seq, 0);
+    return few;
+}
+
 // The scored attention of prompts and single tokens (parents nullptr) and of drafted trees.
 void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* k, const void* v, int in_dtype,
                         int num_kv_heads, const int32_t* streams_host, const int32_t* rows_host, int n_seq,
@@ -596,7 +620,8 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
             "max_period must be above 1, or 0 for no rotation");
     const ptts_b200_scores none{};
     const ptts_b200_scores& sc = scores ? *scores : none;
-    require(sc.softcap >= 0.0f && std::isfinite(sc.softcap), PTTS_B200_ERR_ARG, "softcap must be 0 (none) or positive");
+    require(sc.softcap == 0.0f || (sc.softcap >= 1e-30f && sc.softcap <= 1e30f), PTTS_B200_ERR_ARG,
+            "softcap must be 0 (none) or within 1e-30 .. 1e30");
     auto aligned = [](const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
     require(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16), PTTS_B200_ERR_ARG,
             "q, k, v and out must be aligned to 16 bytes");
@@ -620,37 +645,44 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
     refuse_capture(s, tree ? "ptts_b200_attend_tree" : "ptts_b200_attend_scored");
     const bool cache_bf16 = kv->dtype == PTTS_B200_BF16;
     const size_t hd = (size_t)kv->heads * kHeadDim;
-    // Single tokens run on the split-KV decode, a row per unit. On a bf16 cache up to 64 rows a sequence
-    // run as blocks split over the keys, longer prompts in tiles of 128 rows; on an f32 cache both in
-    // tiles of 32 rows.
-    const int most = *std::max_element(rows_host, rows_host + n_seq);
-    const bool tokens = !tree && n_rows == n_seq, few = !tokens && cache_bf16 && most <= kTreeNodes;
-    const bool prompt = !tokens && cache_bf16 && !few, out_bf16 = out_dtype == PTTS_B200_BF16;
-    int grid = sm_count(kv->device);
-    std::vector<int2> blocks;
-    if (prompt) blocks = make_tiles(offsets, streams_host, kv->h_len);
+    // Single tokens run on the split-KV decode, a row per unit. On a bf16 cache sequences of few rows run
+    // as blocks of up to 64 rows split over the keys (`few`), longer ones in tiles of 128 rows (`prompt`); a
+    // call may have both. On an f32 cache all run in tiles of 32 rows.
+    const bool tokens = !tree && n_rows == n_seq, out_bf16 = out_dtype == PTTS_B200_BF16;
+    const int sms = sm_count(kv->device);
+    std::vector<int2> blocks;  // the rows kernel's blocks, then the prompt (or f32) kernel's tiles
+    int most = 0, grid = sms;  // rows of a block at most; CTAs along the keys
+    const std::vector<char> is_few = tokens || !cache_bf16 ? std::vector<char>(n_seq, 0)
+                                                           : few_row_sequences(kv, streams_host, rows_host, n_seq, tree);
+    for (int i = 0; i < n_seq; ++i)
+        for (int r = offsets[i]; is_few[i] && r < offsets[i + 1]; r += kTreeNodes) {
+            blocks.push_back(make_int2(r, std::min(kTreeNodes, offsets[i + 1] - r)));
+            most = std::max(most, blocks.back().y);
+        }
+    const int n_few = (int)blocks.size();
+    if (n_few) grid = score_rows_grid(out_bf16, kv->heads, sms);
     if (!tokens && !cache_bf16)
         for (int i = 0; i < n_seq; ++i)
             for (int r = offsets[i]; r < offsets[i + 1]; r += kScoreF32Rows)
                 blocks.push_back(make_int2(r, std::min(kScoreF32Rows, offsets[i + 1] - r)));
-    if (few) {
-        grid = score_rows_grid(out_bf16, kv->heads, grid);
-        for (int i = 0; i < n_seq; ++i) blocks.push_back(make_int2(offsets[i], rows_host[i]));
-    }
+    if (!tokens && cache_bf16)
+        for (const int2& t : make_tiles(offsets, streams_host, kv->h_len)) {
+            const size_t i = std::upper_bound(offsets.begin(), offsets.end(), t.x) - offsets.begin() - 1;
+            if (!is_few[i]) blocks.push_back(t);
+        }
+    const int n_tiles = (int)blocks.size() - n_few;
+    const bool few = n_few > 0, prompt = !tokens && cache_bf16 && n_tiles > 0;
     std::vector<int32_t> packed(streams_host, streams_host + n_seq);
     packed.insert(packed.end(), offsets.begin(), offsets.end());
     const size_t blocks_at = append_tiles(packed, blocks);
     const bool inlined = packed.size() <= (size_t)kScoreInline;
-    const int n_units = few ? n_seq : tokens ? n_rows : 0;
-    long long keys = 0;
+    const int n_units = few ? n_few : tokens ? n_rows : 0;
     int most_keys = 0;
-    for (int i = 0; i < n_seq; ++i) {
-        keys += kv->h_len[streams_host[i]] + rows_host[i];
-        most_keys = std::max(most_keys, kv->h_len[streams_host[i]] + rows_host[i]);
-    }
-    const int splits = !tokens && !cache_bf16 ? score_f32_splits((int)blocks.size(), kv->heads, most_keys, grid) : 1;
+    for (int i = 0; i < n_seq; ++i) most_keys = std::max(most_keys, kv->h_len[streams_host[i]] + rows_host[i]);
+    const long long few_keys = (long long)n_few * most_keys;  // at most
+    const int splits = !tokens && !cache_bf16 ? score_f32_splits(n_tiles, kv->heads, most_keys, sms) : 1;
     const size_t part_floats = tokens ? decode_part_floats(n_rows, grid) * kv->groups()
-                               : few  ? score_rows_part_floats(kv->heads, grid, keys, most)
+                               : few  ? score_rows_part_floats(kv->heads, grid, few_keys, most)
                                       : splits > 1 ? (size_t)kPartStride * splits * kv->heads * n_rows : 0;
     // The scratch, cut into 256-byte aligned parts.
     size_t bytes = 0;
@@ -778,7 +810,6 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
         require(launch_score_rows(a, grid, s), PTTS_B200_ERR_CUDA,
                 "could not describe the cache's tensors (cuTensorMapEncodeTiled)");
         check_launch();
-        return;
     }
     if (prompt) {
         ScorePromptArgs a{};
@@ -796,18 +827,18 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
         a.rows = p.rows;
         a.rule.cap = sc.softcap;
         a.rule.slopes = sc.slopes;
-        a.tiles = d_blocks;
-        a.n_tiles = (int)blocks.size();
+        a.tiles = d_blocks + n_few;
+        a.n_tiles = n_tiles;
         // Several heads a CTA share its start and fetch ahead across heads, as long as every SM's two
         // CTAs still get two or more to even out.
         a.heads_per_cta = kGroupHeads;
-        while (a.heads_per_cta > 1 && (long long)a.n_tiles * (kv->heads / a.heads_per_cta) < 4LL * grid) a.heads_per_cta /= 2;
+        while (a.heads_per_cta > 1 && (long long)a.n_tiles * (kv->heads / a.heads_per_cta) < 4LL * sms) a.heads_per_cta /= 2;
         a.err = p.err;
         require(launch_score_prompt(a, s), PTTS_B200_ERR_CUDA,
                 "could not describe the prompt attention's tensors (cuTensorMapEncodeTiled)");
         check_launch();
-        return;
     }
+    if (cache_bf16) return;
     ScoreF32Args a{};
     a.k_cache = p.k_cache;
     a.v_cache = p.v_cache;
@@ -822,7 +853,7 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
     a.rule.cap = sc.softcap;
     a.rule.slopes = sc.slopes;
     a.tiles = d_blocks;
-    a.n_tiles = (int)blocks.size();
+    a.n_tiles = n_tiles;
     a.splits = splits;
     a.part = records;
     launch_score_f32(a, s);

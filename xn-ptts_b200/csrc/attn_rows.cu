@@ -222,8 +222,9 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
                 R->hi[key] = hi;
                 R->pos[key] = (float)pos;
                 R->lineage[key] = there && a.rows.lineage ? a.rows.lineage[row] : 0;
-                // BOUNDED: exp2 against the bias of the nearest visible key. Else the row's first scores set m.
-                R->m[key] = BOUNDED ? -slope * (float)max(max(lo - pos, pos - hi), 0) : 0.f;
+                // BOUNDED: exp2 against the row's greatest bias (a node sees positions lo .. its own). Else the
+                // row's first scores set m.
+                R->m[key] = BOUNDED && biased ? most_bias(slope, pos, lo, a.rows.lineage ? min(hi, pos) : hi) : 0.f;
                 R->has[key] = lo > hi;
             }
             bool fresh = !BOUNDED;  // some row has no maximum yet

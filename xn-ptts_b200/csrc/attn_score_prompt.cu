@@ -14,8 +14,8 @@
 //              in two-slot rings, so the next head's data come during this head's last item.
 // Two threads a row and two CTAs an SM make four softmax warps a scheduler, which fill each other's
 // waits (with a thread a row, half as many, the issue slots were 35 to 46 % used). Where a cap up to
-// kScoreBoundedCap bounds the scores there is no maximum: exp2 runs against the bias of the row's nearest
-// key, which a score passes by at most cap x log2(e) < 58 either way. Items run from the last keys to
+// kScoreBoundedCap bounds the scores there is no maximum: exp2 runs against the row's greatest
+// bias, which a score passes by at most cap x log2(e) < 58 either way. Items run from the last keys to
 // the first: a causal row's nearest keys, whose bias is the least, set the maximum at once.
 //
 // f32 outputs hold P as a bf16 hi/lo pair over the columns of S (its next item waits for P V);
@@ -235,8 +235,7 @@ __global__ void __launch_bounds__(kThreadsP, 2) score_prompt_kernel(ScorePromptA
             const int head = head0 + hh;
             if (kt == 0) {
                 if (BIAS) slope = a.rule.slopes[head] * kScoreLog2e;
-                // BOUNDED: exp2 against the bias of the nearest visible key.
-                m = BOUNDED ? (BIAS ? -slope * (float)max(max(lo - pos, pos - hi), 0) : 0.f) : kScoreLow;
+                m = BOUNDED ? (BIAS ? most_bias(slope, pos, lo, hi) : 0.f) : kScoreLow;
                 l = 0.f;
             }
             const int k0 = first + (n - 1 - kt) * KT, mine = k0 + 64 * half;  // this thread's first key

@@ -115,4 +115,12 @@ __device__ __forceinline__ void clean_v(unsigned char* tile, int key, int c0, bo
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// The greatest bias (in log2 units) of a row at `pos` over its visible positions from .. to: the nearest
+// one's, or the farthest one's where the slope is negative. 0 for a row that sees nothing.
+__device__ __forceinline__ float most_bias(float slope, int pos, int from, int to) {
+    if (from > to) return 0.f;
+    const int near = max(max(from - pos, pos - to), 0), far = max(abs(pos - from), abs(pos - to));
+    return -slope * (float)(slope < 0.f ? far : near);
+}
+
 }  // namespace ptts

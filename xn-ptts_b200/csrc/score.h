@@ -94,15 +94,15 @@ struct ScoreF32Args {
 int score_f32_splits(int tiles, int heads, int most_keys, int sms);
 void launch_score_f32(const ScoreF32Args& a, cudaStream_t s);
 
-// How the matrix-product kernels cap scores: not, by the fast form (bf16 outputs, caps up to
-// kScoreFastCap; q is then scaled by 1 / (8 cap)) or by tanhf (q scaled by log2(e) / 8, as
+// How the matrix-product kernels cap scores: not, by the fast form (bf16 outputs, caps from 1e-3
+// to kScoreFastCap; q is then scaled by 1 / (8 cap)) or by tanhf (q scaled by log2(e) / 8, as
 // without a cap).
 enum { kCapNone = 0, kCapFast = 1, kCapExact = 2 };
 constexpr float kScoreFastCap = 128.f;
 // Caps this small bound the scores: 40 log2(e) < 58, and weights and sums of 2^58 stay far inside f32 and bf16.
 constexpr float kScoreBoundedCap = 40.f;
 inline int score_cap_mode(float cap, bool out_f32) {
-    return cap == 0.f ? kCapNone : (!out_f32 && cap <= kScoreFastCap ? kCapFast : kCapExact);
+    return cap == 0.f ? kCapNone : (!out_f32 && cap >= 1e-3f && cap <= kScoreFastCap ? kCapFast : kCapExact);
 }
 inline float score_q_scale(float cap, bool out_f32) {
     constexpr float log2e = 1.4426950408889634f;
