@@ -22,6 +22,7 @@ from __future__ import annotations
 import ctypes
 import os
 from dataclasses import dataclass, field
+from itertools import chain
 from typing import Optional, Sequence
 
 import numpy as np
@@ -402,11 +403,9 @@ class KvState:
         if len(nodes) != len(streams):
             raise PttsError(ERR_ARG, "one path per stream")
         st, counts = _vec32(streams), np.fromiter(map(len, nodes), np.int32, len(nodes))
-        try:  # node indexes are below 64: lists of them flatten fastest as bytes
-            if not set(map(type, nodes)) <= {list, tuple}:
-                raise ValueError
-            flat = np.frombuffer(b"".join(map(bytes, nodes)), np.uint8).astype(np.int32)
-        except (ValueError, TypeError):  # other sequences, or indexes that the library will refuse
+        try:  # node indexes are below 64: a batch of paths flattens fastest as bytes
+            flat = np.frombuffer(bytes(chain.from_iterable(nodes)), np.uint8).astype(np.int32)
+        except (ValueError, TypeError):  # an index that the library will refuse
             flat = _i32([x for path in nodes for x in path])
         _check(lib().ptts_b200_kv_accept(self._h, st.ctypes.data, counts.ctypes.data, flat.ctypes.data, st.size,
                                          _stream_of(self.device, stream)))
