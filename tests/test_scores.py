@@ -527,6 +527,39 @@ def test_draft_accept_and_go_on_equals_one_row_at_a_time(ptts, cuda, heads, dtyp
     b.kv.check(), c.kv.check()
 
 
+# ---- large offsets --------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("kind", ["tokens", "prompts", "trees"])
+def test_offsets_past_32_bits(ptts, cuda, kind, dtype):
+    """Five streams of over a million slots: the last one's rows lie past 2^32 bytes (and 2^31 elements) of
+    the cache, and the long stream's own keys past 2^30. Its weights' sum has 2^9 f32 steps (the parts'
+    chunks and their joining, at most 2^8 of either): 2^-15 in place of the module's 2^-18."""
+    import torch
+    rows = {"tokens": [1] * 5, "prompts": [5, 200, 70, 1, 33], "trees": [9, 64, 1, 33, 17]}[kind]
+    b = Batch(ptts, cuda, [1_100_000, 700, 0, 40, 900], rows, dtype=dtype, spare=0, seed=21, tree=kind == "trees")
+    assert 4 * b.capacity * 512 > 2 ** 31
+    args = dict(softcap=20.0, slopes=b.slopes)
+    if kind == "trees":
+        out = ptts.attend_tree(b.kv, 0, b.q, b.k, b.v, b.streams, b.rows, b.parents_dev, **args)
+    else:
+        out = ptts.attend_scored(b.kv, 0, b.q, b.k, b.v, b.streams, b.rows, **args)
+    b.kv.check()
+    want, bound = b.want(tree=kind == "trees", half_p=PAIR_HALF + 2.0 ** -15, **args)
+    compare(out, want, bound)
+    b.check_rows(tree=kind == "trees")
+    if kind != "trees":
+        return
+    kt, vt, _ = b.kv.tensors(0)
+    paths = [sorted(lineages(p)[1][-1]) for p in b.parents]
+    kept = [[t[int(st), [int(L) + i for i in p]].clone() for t in (kt, vt)] for st, L, p in zip(b.streams, b.cached, paths)]
+    b.kv.accept(b.streams, paths)
+    for st, L, p, rows in zip(b.streams, b.cached, paths, kept):
+        for t, r in zip((kt, vt), rows):
+            assert torch.equal(t[int(st), int(L):int(L) + len(p)], r)
+
+
 # ---- refusals ---------------------------------------------------------------------------------------
 
 def test_null_handles_are_refused_without_a_device(ptts):
