@@ -696,7 +696,9 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
                  at_lineage = part(tree ? sizeof(unsigned long long) * (size_t)n_rows : 0),
                  at_units = part(n_units ? sizeof(int32_t) * (2 * (size_t)n_units + 1 + grid) : 0),
                  at_part = part(sizeof(float) * part_floats);
-    char* ws = static_cast<char*>(kv->score.need(bytes));
+    // Grown by half at a time, from 1 MB: a cache that fills up row by row does not allocate row by row.
+    if (bytes > kv->score.bytes) kv->score.need(std::max({bytes, kv->score.bytes / 2 * 3, (size_t)1 << 20}));
+    char* ws = static_cast<char*>(kv->score.p);
     // A short list rides in the plan's parameters, and the plan leaves it in the scratch for the kernels
     // after it.
     ScoreInline in;
