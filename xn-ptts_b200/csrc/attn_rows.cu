@@ -22,6 +22,10 @@
 //   warps 8, 9      one lane each issues a head's MMAs; the next item's S starts when this one's scores
 //                   are in registers.
 //   warp 10         one lane copies the heads' Q tiles and K and V items by TMA, two slots each.
+// Measured (one B200, 8 heads, bf16): 128 streams of 64-2048 cached rows with trees of 8-64 nodes, cap 30,
+// 107 us of the kernel's own (an item 3500 cycles, 2800 at HBM's rate; a block's start and end 5000-10000
+// that nothing overlaps); 4 full trees over 20000-33000 rows, 87 us a call. The same split with rows as M
+// on mma.sync: 213 and 125 us a call against 129 and 87.
 // A block inside one CTA's range is written at once; the pieces of a cut block leave (max, sum, acc)
 // records that a second kernel joins, one warp per row and head: 64 rows x 8 heads are too many for
 // the warp that finishes last.

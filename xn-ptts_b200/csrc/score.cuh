@@ -39,7 +39,7 @@ __device__ __forceinline__ float cap_exact(float x, float cap) {
 // that fits it best (least largest error, 3.6e-6) on |y| <= 3/4, fitted to numpy's tanh by reweighted
 // least squares; where some score of the warp is past that, tanh(y) = 1 - 2 / (1 + e^2y) by one exp2
 // and one reciprocal, whose difference cancels near 0 (an absolute error near 2^-20). Either moves a
-// weight by less than 2^-10 for cap <= kScoreFastCap, half of bf16's own half step of 2^-9.
+// weight by less than 2^-10 for cap <= kScoreFastCap, a quarter of bf16's own half step of 2^-8.
 // On the packed FMAs the polynomial costs 5 pipe cycles a score, the other form 2 of the 3 operations
 // at exp2's rate (8 cycles each) that would then bound a capped softmax.
 template <int N>

@@ -6,7 +6,9 @@
 // warp per row, whose lanes compute the 32 pairs' sines and cosines once for all heads.
 //
 // Bound by memory for prompts (per row (H + 2 KVH) x 64 inputs read, H x 64 x 2 cache elements and
-// the q planes written) and by launch latency for single tokens.
+// the q planes written) and by launch latency for single tokens. Measured (one B200): 54,073 rows of
+// 8 heads, 388 MB, 88 us, 67 % of a copy's rate; fetching a row's q, k and v ahead of the rotation 102,
+// registers bounded for 5 or 6 CTAs an SM 97, for 8 126.
 #include "common.cuh"
 #include "score.h"
 
