@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
                     ld16(lanes + 64 + 16 * g, o);
                     fa_wait_ld();
                     if (bad) add_not_finite(a, *R, w, base_slot, head, key, 16 * g, o);
-const int rows = w.nrows - 16 * g;  // of these 16
+                    const int rows = w.nrows - 16 * g;  // of these 16
                     if (w.whole) {
                         using Out = typename std::conditional<P2, float, __nv_bfloat16>::type;
                         Out* out = static_cast<Out*>(a.out) + at + (long long)(16 * g) * a.ld;
@@ -546,6 +546,24 @@ const int rows = w.nrows - 16 * g;  // of these 16
         // ---- producer -------------------------------------------------------------------------------
         bool ok = true;
         int i = 0, piece = 0, q_out = 0, k_out = 0, v_out = 0;  // copies are issued for all heads up to these
+        // Item j's keys or values: its 128 rows of the cache from row `at` on.
+        auto copy = [&](bool value, int j, int at) {
+            const int slot = j % kSlots;
+            for (int hl = 0; hl < HC && ok; ++hl) {
+                HeadBars* b = bars_of(hl);
+                const int head = head0 + hl;
+                if (j >= kSlots && !(ok = mbar_wait(value ? &b->vempty[slot] : &b->kempty[slot], ((j / kSlots) & 1) ^ 1))) break;
+                uint64_t* full = value ? &b->vfull[slot] : &b->kfull[slot];
+                mbar_arrive_expect_tx(full, kTile);
+                fa_tma(base + (value ? L::kV : L::kK) + (hl * kSlots + slot) * kTile, value ? &tm_v : &tm_k,
+                       head % kGroupHeads * kHeadDim, head / kGroupHeads * a.num_streams * a.capacity + at, full);
+                (value ? v_out : k_out) = j * HC + hl + 1;
+            }
+        };
+        // An item's values come after the next item's keys: their slot is free an item later (P V ends where
+        // the next softmax begins, S before it), and keys behind that wait would have one item's time to
+        // arrive, not two.
+        int before = 0;  // where the item before begins
         Walk w(a, c, total, G);
         for (; ok && w.next(); ++piece) {
             const int sid = max(a.rows.stream[w.row0], 0);  // a refused tree reads slot 0 and sees nothing
@@ -558,24 +576,14 @@ const int rows = w.nrows - 16 * g;  // of these 16
                 fa_tma(q + kQTile, &tm_ql, (head0 + hl) * kHeadDim, w.row0, &b->qready);
                 q_out = piece * HC + hl + 1;
             }
-            const int n = w.items();
+            const int n = w.items(), first = sid * a.capacity + w.lo + w.s0;
             for (int it = 0; it < n && ok; ++it, ++i) {
-                const int slot = i % kSlots;
-                const uint32_t ph = ((i / kSlots) & 1) ^ 1;
-                for (int kv = 0; kv < 2 && ok; ++kv)
-                    for (int hl = 0; hl < HC && ok; ++hl) {
-                        HeadBars* b = bars_of(hl);
-                        const int head = head0 + hl;
-                        const int y = (int)(((long long)(head / kGroupHeads) * a.num_streams + sid) * a.capacity) + w.lo + w.s0 + it * KT;
-                        if (i >= kSlots && !(ok = mbar_wait(kv ? &b->vempty[slot] : &b->kempty[slot], ph))) break;
-                        uint64_t* full = kv ? &b->vfull[slot] : &b->kfull[slot];
-                        mbar_arrive_expect_tx(full, kTile);
-                        fa_tma(base + (kv ? L::kV : L::kK) + (hl * kSlots + slot) * kTile, kv ? &tm_v : &tm_k,
-                               head % kGroupHeads * kHeadDim, y, full);
-                        (kv ? v_out : k_out) = i * HC + hl + 1;
-                    }
+                copy(false, i, first + it * KT);
+                if (i > 0 && ok) copy(true, i - 1, before);
+                before = first + it * KT;
             }
         }
+        if (i > 0 && ok) copy(true, i - 1, before);
         if (!ok) set_error(a.err, DEV_ERR_TIMEOUT);
         // The last copies into each buffer land before the shared memory goes (a completed phase returns at
         // once). Copy j of a kind is head j % HC's item (or piece) j / HC.

@@ -446,6 +446,17 @@ __global__ void __launch_bounds__(kThreadsP, 2) score_prompt_kernel(ScorePromptA
     } else if (warp == kLoadW && lane == 0) {
         // ---- Q, K and V producer -----------------------------------------------------------------
         bool ok = true;
+        // An item's values come after the next item's keys: their slot is free an item later (P V ends where
+        // the next softmax begins, S before it), and keys behind that wait would have one item's time to
+        // arrive, not two.
+        int v_x = 0, v_y = 0;  // the item before
+        auto copy_v = [&](int i, int x, int y) {
+            const int slot = i % kSlots;
+            if (i >= kSlots && !(ok = mbar_wait(&b->vempty[slot], ((i / kSlots) & 1) ^ 1))) return;
+            mbar_arrive_expect_tx(&b->vfull[slot], kTile);
+            fa_tma(base + kOffV + slot * kTile, &tm_v, x, y, &b->vfull[slot]);
+            s_v_issued = i + 1;
+        };
         for (int i = 0, kt = 0, hh = 0; i < items && ok; ++i) {
             const int slot = i % kSlots, head = head0 + hh, y = kv_row(head) + first + (n - 1 - kt) * KT;
             if (kt == 0) {
@@ -466,12 +477,11 @@ __global__ void __launch_bounds__(kThreadsP, 2) score_prompt_kernel(ScorePromptA
             mbar_arrive_expect_tx(&b->kfull[slot], kTile);
             fa_tma(base + kOffK + slot * kTile, &tm_k, kv_x(head), y, &b->kfull[slot]);
             s_k_issued = i + 1;
-            if (i >= kSlots && !(ok = mbar_wait(&b->vempty[slot], ((i / kSlots) & 1) ^ 1))) break;
-            mbar_arrive_expect_tx(&b->vfull[slot], kTile);
-            fa_tma(base + kOffV + slot * kTile, &tm_v, kv_x(head), y, &b->vfull[slot]);
-            s_v_issued = i + 1;
+            if (i > 0) copy_v(i - 1, v_x, v_y);
+            v_x = kv_x(head), v_y = y;
             if (++kt == n) kt = 0, ++hh;
         }
+        if (ok && items > 0) copy_v(items - 1, v_x, v_y);
         if (!ok) set_error(a.err, DEV_ERR_TIMEOUT);
     }
     fa_before();
