@@ -585,21 +585,23 @@ void refuse_capture(cudaStream_t s, const char* what) {
 // however few its rows, and the GPU 0.000305 a tile and key once it is full; the rows kernel takes 0.0005 a
 // block and key, and 14 more to start and join. So a sequence whose tile alone would outlast the whole
 // call's tiles by that goes there (one of 65 rows on 8000 keys: 38 against 102; single tokens beside a
-// prompt), unless all that went there would take longer than its longest tile.
+// prompt), unless all that went there would take longer than its longest tile, or
+// its keys' costs would pass the plan's 32 bits.
 std::vector<char> few_row_sequences(const ptts_b200_kv* kv, const int32_t* streams, const int32_t* rows, int n_seq,
                                     bool tree) {
     std::vector<char> few(n_seq, tree);
     if (tree) return few;
     const double per_tile = 0.0113, full = 0.000305 * kv->groups(), per_block = 0.0005 * kv->groups(), start = 14.0;
-    double all = 0.0, blocks = start, longest = 0.0;
+    double all = 0.0, blocks = start, longest = 0.0, block_keys = 0.0;
     auto keys = [&](int i) { return (double)kv->h_len[streams[i]] + rows[i]; };
     for (int i = 0; i < n_seq; ++i) all += full * ((rows[i] + 127) / 128) * keys(i);
     for (int i = 0; i < n_seq; ++i)
         if ((few[i] = per_tile * keys(i) > all + start)) {
             blocks += per_block * ((rows[i] + kTreeNodes - 1) / kTreeNodes) * keys(i);
+            block_keys += (rows[i] + kTreeNodes - 1) / kTreeNodes * keys(i);
             longest = std::max(longest, per_tile * keys(i));
         }
-    if (blocks > longest) few.assign(n_seq, 0);
+    if (blocks > longest || block_keys > 2e8) few.assign(n_seq, 0);
     return few;
 }
 
@@ -682,7 +684,7 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
     const long long few_keys = (long long)n_few * most_keys;  // at most
     const int splits = !tokens && !cache_bf16 ? score_f32_splits(n_tiles, kv->heads, most_keys, sms) : 1;
     const size_t part_floats = tokens ? decode_part_floats(n_rows, grid) * kv->groups()
-                               : few  ? score_rows_part_floats(kv->heads, grid, few_keys, most)
+                               : few  ? score_rows_part_floats(kv->heads, grid, few_keys, n_few, most)
                                       : splits > 1 ? (size_t)kPartStride * splits * kv->heads * n_rows : 0;
     // The scratch, cut into 256-byte aligned parts.
     size_t bytes = 0;

@@ -113,17 +113,21 @@ struct Walk {
     __device__ Walk(const ScoreRowsArgs& a_, int c, long long total, int G)
         : a(a_), start(cta_start(c, total, G)), end(cta_start(c + 1, total, G)), u(a_.cta_first[c] - 1) {}
     __device__ bool next() {
-        if (++u >= a.n_units) return false;
-        const long long pb = a.prefix[u], pe = a.prefix[u + 1];
-        if (pb >= end) return false;
-        s0 = (int)((start > pb ? start : pb) - pb);
-        s1 = (int)((end < pe ? end : pe) - pb);
-        begins = pb >= start;
-        whole = begins && pe <= end;
-        lo = a.unit_lo[u];
-        row0 = a.blocks[u].x;
-        nrows = a.blocks[u].y;
-        return true;
+        while (++u < a.n_units) {
+            const long long pb = a.prefix[u], pe = a.prefix[u + 1];
+            if (pb >= end) return false;
+            row0 = a.blocks[u].x;
+            nrows = a.blocks[u].y;
+            const unsigned cost = score_key_cost(nrows), keys = (unsigned)(pe - pb - kScoreBlockCost) / cost;
+            s0 = start > pb ? (int)min(keys, (unsigned)(start - pb) / cost) : 0;
+            s1 = (int)min(keys, (unsigned)(end - pb) / cost);
+            if (s0 >= s1) continue;  // its keys are other CTAs'
+            begins = s0 == 0;
+            whole = begins && s1 == (int)keys;
+            lo = a.unit_lo[u];
+            return true;
+        }
+        return false;
     }
     __device__ int items() const { return (s1 - s0 + KT - 1) / KT; }
 };
@@ -196,7 +200,7 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
     grid_dep_wait();
     grid_dep_launch();
     const long long total = a.prefix[a.n_units];
-    const int G = ctas_in_use(total, gridDim.x), c = blockIdx.x;
+    const int G = score_ctas(total, gridDim.x), c = blockIdx.x;
     const int head0 = blockIdx.y * HC;
     const bool idle = c >= G;
 
@@ -609,11 +613,12 @@ __global__ void __launch_bounds__(256) score_rows_merge_kernel(ScoreRowsArgs a, 
     grid_dep_wait();
     grid_dep_launch();
     const long long total = a.prefix[a.n_units];
-    const int G = ctas_in_use(total, grid), u = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 31;
+    const int G = score_ctas(total, grid), u = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 31;
     const long long pb = a.prefix[u], pe = a.prefix[u + 1];
-    const int c0 = cta_of(pb, total, G), c1 = cta_of(pe - 1, total, G);
-    if (c0 == c1) return;
     const int2 rows = a.blocks[u];
+    // The CTAs that hold its first key and its last (see Walk).
+    const int c0 = cta_of(pb + score_key_cost(rows.y) - 1, total, G), c1 = cta_of(pe - kScoreBlockCost - 1, total, G);
+    if (c0 == c1) return;
     const int r = blockIdx.z * 8 + (threadIdx.x >> 5);
     if (r >= rows.y) return;
     auto rec = [&](int c) {
@@ -670,9 +675,9 @@ int score_rows_grid(bool out_bf16, int heads, int sms) {
     return sms / slabs > 1 ? sms / slabs : 1;
 }
 
-size_t score_rows_part_floats(int heads, int grid, long long keys, int most_rows) {
-    const long long ctas = (keys + kMinKeysPerCta - 1) / kMinKeysPerCta;  // ctas_in_use, at most
-    return (size_t)2 * (ctas < grid ? ctas : grid) * heads * most_rows * kPartStride;
+size_t score_rows_part_floats(int heads, int grid, long long keys, int blocks, int most_rows) {
+    const long long ctas = score_ctas(keys * score_key_cost(kTreeNodes) + (long long)blocks * kScoreBlockCost, grid);  // at most
+    return (size_t)2 * ctas * heads * most_rows * kPartStride;
 }
 
 bool launch_score_rows(const ScoreRowsArgs& a, int grid, cudaStream_t s) {

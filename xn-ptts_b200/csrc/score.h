@@ -67,6 +67,15 @@ struct ScorePlanArgs {
     int grid = 0;
     uint32_t* err;
 };
+// What the partition of blocks counts: a key costs 3 and 1 more for each 16 rows that score it (its bytes,
+// then its softmax: 128 keys of a head pair take 1.2 us at 16 rows and 2.1 at 64), a block kScoreBlockCost
+// behind its keys (rows and masks read, sums and records written, 4 to 6 us).
+constexpr int kScoreBlockCost = 2560;
+__host__ __device__ constexpr int score_key_cost(int rows) { return 3 + (rows + 15) / 16; }
+__host__ __device__ inline int score_ctas(long long total, int grid) {  // at least 32 keys a CTA
+    const long long g = (total + 127) / 128;
+    return (int)(g < 1 ? 1 : (g > grid ? grid : g));
+}
 constexpr int kScoreInline = 768;
 struct ScoreInline {  // a short list rides in the launch's parameters
     int32_t list[kScoreInline];
@@ -131,8 +140,8 @@ struct ScoreRowsArgs {
     uint32_t* err;
 };
 int score_rows_grid(bool out_bf16, int heads, int sms);  // CTAs along the keys (the plan's grid)
-// For `keys` keys of all blocks (an upper bound) and blocks of up to most_rows rows.
-size_t score_rows_part_floats(int heads, int grid, long long keys, int most_rows);
+// For `keys` keys of all blocks (an upper bound).
+size_t score_rows_part_floats(int heads, int grid, long long keys, int blocks, int most_rows);
 bool launch_score_rows(const ScoreRowsArgs& a, int grid, cudaStream_t s);
 
 // Prompts on tcgen05, bf16 caches (attn_score_prompt.cu): tiles (first row, rows) of up to 128

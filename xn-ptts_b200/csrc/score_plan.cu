@@ -104,6 +104,7 @@ __device__ __forceinline__ void plan_units(const ScorePlanArgs& a, const int32_t
                 a.unit_lo[u] = lo;
                 v = max(hi - lo + 1, 1);
             }
+            if (blocks) v = v * score_key_cost(unit(u).y) + kScoreBlockCost;
         }
         int x = v;
 #pragma unroll
@@ -121,7 +122,7 @@ __device__ __forceinline__ void plan_units(const ScorePlanArgs& a, const int32_t
         __syncthreads();
     }
     const long long total = carry;
-    const int G = ctas_in_use(total, a.grid);
+    const int G = blocks ? score_ctas(total, a.grid) : ctas_in_use(total, a.grid);
     for (int u = tid; u < a.n_units; u += kPlanThreads) {
         const long long pb = a.prefix[u], pe = a.prefix[u + 1];
         for (int c = cta_of(pb, total, G); c <= cta_of(pe - 1, total, G); ++c)
