@@ -608,17 +608,22 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
 
 // Joins the pieces of the blocks that CTAs' ranges cut: one warp per row and head, lane = 2 dims.
 // Every warp reads the pieces' maxima and sums lane by lane and then all records at once.
-template <bool P2>
+// A grid over the blocks, or where they are more than the CTAs' ranges (BY_CUT) over the ranges' beginnings:
+// 128 blocks cut by 37 ranges, 115 us a call over the blocks, 110 over the beginnings.
+template <bool P2, bool BY_CUT>
 __global__ void __launch_bounds__(256) score_rows_merge_kernel(ScoreRowsArgs a, int grid) {
     grid_dep_wait();
     grid_dep_launch();
     const long long total = a.prefix[a.n_units];
-    const int G = score_ctas(total, grid), u = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 31;
+    const int G = score_ctas(total, grid), head = blockIdx.y, lane = threadIdx.x & 31;
+    const int cut = BY_CUT ? (int)blockIdx.x + 1 : 0;  // CTA `cut`'s range begins in the block, and is its first such
+    if (cut >= G) return;
+    const int u = BY_CUT ? a.cta_first[cut] : blockIdx.x;
     const long long pb = a.prefix[u], pe = a.prefix[u + 1];
     const int2 rows = a.blocks[u];
     // The CTAs that hold its first key and its last (see Walk).
     const int c0 = cta_of(pb + score_key_cost(rows.y) - 1, total, G), c1 = cta_of(pe - kScoreBlockCost - 1, total, G);
-    if (c0 == c1) return;
+    if (c0 == c1 || (BY_CUT && cut != c0 + 1)) return;
     const int r = blockIdx.z * 8 + (threadIdx.x >> 5);
     if (r >= rows.y) return;
     auto rec = [&](int c) {
@@ -654,8 +659,10 @@ __global__ void __launch_bounds__(256) score_rows_merge_kernel(ScoreRowsArgs a, 
 
 template <bool P2>
 void merge(const ScoreRowsArgs& a, int grid, cudaStream_t s) {
-    if (grid > 1)
-        launch_k(score_rows_merge_kernel<P2>, dim3(a.n_units, a.heads, (a.most_rows + 7) / 8), dim3(256), 0, s, a, grid);
+    if (grid == 1) return;
+    const bool by_cut = a.n_units >= grid;
+    launch_k(by_cut ? score_rows_merge_kernel<P2, true> : score_rows_merge_kernel<P2, false>,
+             dim3(by_cut ? grid - 1 : a.n_units, a.heads, (a.most_rows + 7) / 8), dim3(256), 0, s, a, grid);
 }
 
 template <int HC, int CAP, bool BOUNDED, bool P2>
