@@ -629,20 +629,20 @@ __global__ void __launch_bounds__(256) score_rows_merge_kernel(ScoreRowsArgs a, 
     auto rec = [&](int c) {
         return a.part + (((long long)(2 * c + (c == c0 ? 1 : 0)) * a.heads + head) * a.most_rows + r) * kPartStride;
     };
-    float mx = kScoreLow;
-    for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, rec(c)[64]);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    float den = 0.f, x0 = 0.f, x1 = 0.f;
-    for (int cb = c0; cb <= c1; cb += 32) {
+    float mx = kScoreLow, den = 0.f, x0 = 0.f, x1 = 0.f;
+    for (int cb = c0; cb <= c1; cb += 32) {  // a lane's piece's maximum and sum, then all its records
         const int n = min(32, c1 - cb + 1);
-        float w = 0.f;
-        if (lane < n) {
-            const float2 ml = *reinterpret_cast<const float2*>(rec(cb + lane) + 64);
-            w = score_exp2(ml.x - mx);
-            den += w * ml.y;
-        }
-#pragma unroll 8
+        float2 ml = make_float2(kScoreLow, 0.f);
+        if (lane < n) ml = *reinterpret_cast<const float2*>(rec(cb + lane) + 64);
+        float top = ml.x;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top = fmaxf(top, mx);
+        const float before = score_exp2(mx - top), w = lane < n ? score_exp2(ml.x - top) : 0.f;
+        mx = top;
+        den = fmaf(w, ml.y, den * before);
+        x0 *= before, x1 *= before;
+#pragma unroll 4
         for (int i = 0; i < n; ++i) {
             const float f = __shfl_sync(0xffffffffu, w, i);
             const float2 v = *reinterpret_cast<const float2*>(rec(cb + i) + 2 * lane);

@@ -242,7 +242,7 @@ __device__ __forceinline__ void plan(const ScorePlanArgs& a, const int32_t* list
     };
     const int mine = lane / (kHeadDim / E), dim = lane % (kHeadDim / E) * E;  // of a step's heads; first dim
     const Tin* q = static_cast<const Tin*>(a.q) + (long long)r * a.heads * kHeadDim + dim;
-#pragma unroll 2
+#pragma unroll 1  // (by two: 1 to 2 us more a call, the code has to be fetched)
     for (int h = mine; h < a.heads; h += HS) {
         const long long at = ((long long)r * a.heads + h) * kHeadDim + dim;
         float x[E];
@@ -267,7 +267,7 @@ __device__ __forceinline__ void plan(const ScorePlanArgs& a, const int32_t* list
     const Tin* v = static_cast<const Tin*>(a.v) + (long long)r * a.kv_heads * kHeadDim + dim;
     T* kc = static_cast<T*>(a.k_cache) + dim;
     T* vc = static_cast<T*>(a.v_cache) + dim;
-#pragma unroll 2
+#pragma unroll 1  // (by two: 1 to 2 us more a call, the code has to be fetched)
     for (int h = mine; h < a.kv_heads; h += HS) {
         float x[E], y[E];
         load_in(k + h * kHeadDim, x);
