@@ -371,6 +371,7 @@ TREES = {
     "batch": ([3, 64, 200, 31, 1000], [16, 17, 64, 1, 33]),
     "long": ([6000, 50], [48, 20]),
     "many": ([(i * 53) % 300 for i in range(260)], [1 + (i * 7) % 64 for i in range(260)]),
+    "uneven": ([0, 3000, 1, 2500, 5, 1800] * 7, [64, 1, 33, 64, 2, 17] * 7),
 }
 
 

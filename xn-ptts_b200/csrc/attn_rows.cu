@@ -11,7 +11,8 @@
 //                   rows' sums of P beside their products, in lane 64
 // At N = 64 that is 4 cycles a key, and the softmax 4 (64 exp2 at 16 a cycle), side by side.
 //
-// Work split as in attn_decode.cu: the blocks' keys lie end to end and every CTA takes an equal range,
+// Work split as in attn_decode.cu: the blocks' keys lie end to end, each at its cost (score.h: ranges of
+// equal keys end 64 to 106 us after their start, of equal cost 73 to 92), and every CTA takes an equal range,
 // for two heads (f32 outputs: one), each head a pipeline of its own:
 //   warps 0-3, 4-7  a thread per key (TMEM lane) of the head's 128-key item, its scores against all rows
 //                   in registers: rules, mask, exp2 against the rows' maxima in shared memory, P^T as
@@ -23,9 +24,9 @@
 //                   are in registers.
 //   warp 10         one lane copies the heads' Q tiles and K and V items by TMA, two slots each.
 // Measured (one B200, 8 heads, bf16): 128 streams of 64-2048 cached rows with trees of 8-64 nodes, cap 30,
-// 107 us of the kernel's own (an item 3500 cycles, 2800 at HBM's rate; a block's start and end 5000-10000
-// that nothing overlaps); 4 full trees over 20000-33000 rows, 87 us a call. The same split with rows as M
-// on mma.sync: 213 and 125 us a call against 129 and 87.
+// 108 us a call, about 85 of them this kernel (an item 1.2 us at 16 rows, 2.1 at 64, 1.46 at HBM's rate; a
+// block's start and end 4-6 that nothing overlaps); 4 full trees over 20000-33000 rows, 78 us a call. Rows
+// as M on mma.sync took 213 and 125 where this form then took 129 and 87.
 // A block inside one CTA's range is written at once; the pieces of a cut block leave (max, sum, acc)
 // records that a second kernel joins, one warp per row and head: 64 rows x 8 heads are too many for
 // the warp that finishes last.

@@ -58,7 +58,8 @@ struct ScorePlanArgs {
     float inv_freq[kMaxPairs];
     ScoreRows rows;
     // Split kernels: the work units (single rows, or blocks of consecutive rows of one sequence:
-    // (first row, rows)), their key counts laid end to end, and the unit each CTA starts in.
+    // (first row, rows)), their key counts (of blocks, their costs) laid end to end, and the unit each CTA
+    // starts in.
     int blocks_at = -1;            // where the blocks are in the list; -1: unit u is row u
     int n_units = 0;               // 0: no units
     int32_t* prefix = nullptr;     // [n_units + 1]
