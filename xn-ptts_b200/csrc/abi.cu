@@ -35,7 +35,7 @@ struct Workspace {
     // persistent linears reread every weight tile for each row tile; widening once per call
     // beats widening every tile on chip). Four matrices, 256-byte aligned slices.
     DevBuf wconv;
-    void size(const ptts_b200_config& c, int rows) {
+    void size(const ptts_b200_config& c, int rows, cudaStream_t s) {
         const size_t r = (size_t)rows, hd = (size_t)c.num_heads * c.head_dim;
         q_rot.need(r * hd * 4);
         h_hi.need(r * c.d_model * 2);
@@ -45,7 +45,7 @@ struct Workspace {
         ff_hi.need(r * c.dim_feedforward * 2);
         ff_lo.need(r * c.dim_feedforward * 2);
         split.need(4 * r * c.d_model * 4);
-        counters.need_zeroed(decode_counter_ints(r) * sizeof(int) * (c.num_heads / kGroupHeads));
+        counters.need_zeroed(decode_counter_ints(r) * sizeof(int) * (c.num_heads / kGroupHeads), s);
     }
 };
 
@@ -496,7 +496,7 @@ void attention_group(const ptts_b200_kv* kv, int layer, int g, bool decode, cons
         a.out_mode = out_mode;
         a.ld = ld;
         a.part = static_cast<float*>(part.need(sizeof(float) * n_part * G)) + n_part * g;
-        a.counters = static_cast<int*>(counters.need_zeroed(sizeof(int) * n_cnt * G)) + n_cnt * g;
+        a.counters = static_cast<int*>(counters.need_zeroed(sizeof(int) * n_cnt * G, s)) + n_cnt * g;
         a.cta_first = plan.cta_first;
         a.B = n_rows;
         a.qscale = qscale;
@@ -701,6 +701,9 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
     // Grown by half at a time, from 1 MB: a cache that fills up row by row does not allocate row by row.
     if (bytes > kv->score.bytes) kv->score.need(std::max({bytes, kv->score.bytes / 2 * 3, (size_t)1 << 20}));
     char* ws = static_cast<char*>(kv->score.p);
+    // The merge counters too come before the plan: a call that finds no memory has changed nothing.
+    int* counters = !tokens ? nullptr
+                            : static_cast<int*>(kv->counters.need_zeroed(sizeof(int) * decode_counter_ints(n_rows) * kv->groups(), s));
     // A short list rides in the plan's parameters, and the plan leaves it in the scratch for the kernels
     // after it.
     ScoreInline in;
@@ -776,7 +779,7 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
             a.out_mode = out_dtype == PTTS_B200_BF16 ? kOutBf16 : kOutF32;
             a.ld = (int)hd;
             a.part = records + n_part * g;
-            a.counters = static_cast<int*>(kv->counters.need_zeroed(sizeof(int) * n_cnt * kv->groups())) + n_cnt * g;
+            a.counters = counters + n_cnt * g;
             a.B = n_rows;
             a.capacity = kv->capacity;
             a.cap = sc.softcap;
@@ -1280,7 +1283,7 @@ void run_step(ptts_b200_model* model, ptts_b200_kv* kv, const int32_t* streams_h
             ln.off = i == 0 ? 0 : n0;
             ln.n = i == 0 ? n0 : n - n0;
             const int r = std::max(ln.n, 1);
-            ln.ws.size(c, r);
+            ln.ws.size(c, r, s);
             ln.ws.part.need(sizeof(float) * decode_part_floats(r, grid) * (c.num_heads / kGroupHeads));
             ln.row_stream.need(sizeof(int32_t) * r);
             ln.row_pos.need(2 * sizeof(int32_t) * r);  // positions, then slots
@@ -2025,7 +2028,7 @@ int ptts_b200_forward(ptts_b200_model* model, ptts_b200_kv* kv, const void* x,
         const RowPlan plan = make_plan(kv, decode, d, d + n_seq, n_seq, rows, model->row_stream,
                                        model->row_pos, model->prefix, s);
         check_launch();
-        model->ws.size(c, rows);
+        model->ws.size(c, rows, s);
         Tiles tiles;
         if (!decode) {
             tiles.dev = reinterpret_cast<const int2*>(d + tile_at);

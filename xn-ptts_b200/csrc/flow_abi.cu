@@ -500,7 +500,7 @@ int ptts_b200_flow_finish(ptts_b200_flow* flow) {
             }
             put(flow->temb, all);
         }
-        flow->err.need_zeroed(sizeof(uint32_t));
+        flow->err.need_zeroed(sizeof(uint32_t), nullptr);
         CK(cudaDeviceSynchronize());
         flow->ready = true;
     });

@@ -104,11 +104,12 @@ struct DevBuf {
     T* as() const {
         return static_cast<T*>(p);
     }
-    // Like need(), and zero-filled whenever it is (re)allocated.
-    void* need_zeroed(size_t n) {
+    // Like need(), and zero-filled whenever it is (re)allocated, on the stream whose kernels use it: a
+    // memset on the legacy default stream is not ordered with a non-blocking stream's work.
+    void* need_zeroed(size_t n, cudaStream_t s) {
         if (n <= bytes) return p;
         need(n);
-        CK(cudaMemset(p, 0, n));
+        CK(cudaMemsetAsync(p, 0, n, s));
         return p;
     }
 };
