@@ -53,7 +53,7 @@ extern "C" {
 
 /* Bits of the device-side error word (ptts_b200_kv_check reads the kv's own word;
  * ptts_b200_attend_decode_noalloc ORs them into the caller's). */
-#define PTTS_B200_DEVERR_BOUNDS 1u    /* a stream index outside the cache's streams */
+#define PTTS_B200_DEVERR_BOUNDS 1u    /* an index outside its range (streams, parents) */
 #define PTTS_B200_DEVERR_CAPACITY 2u  /* a row's position outside its stream's slots */
 #define PTTS_B200_DEVERR_TIMEOUT 4u   /* a bounded wait inside a kernel gave up */
 #define PTTS_B200_DEVERR_DUPLICATE 8u /* a stream named by two rows of one decode call */
@@ -240,7 +240,11 @@ typedef struct {
  * max_period 0 leaves q and k unrotated (for a distance bias in place of RoPE).
  * q, k, v and out are aligned to 16 bytes. Streams are appended streams (rings and windowed
  * streams are refused with PTTS_B200_ERR_UNSUPPORTED), and the call cannot be captured in a CUDA
- * graph (PTTS_B200_ERR_STATE): it plans from the host's lengths. Lengths are not advanced. */
+ * graph (PTTS_B200_ERR_STATE): it plans from the host's lengths. Lengths are not advanced.
+ * Rows are placed by the device's lengths. Where those are not the host's any more (a caller's graph
+ * that advances, a caller that writes them) a sequence that does not fit its stream there is refused on
+ * the device (PTTS_B200_DEVERR_CAPACITY in ptts_b200_kv_check): nothing is written to its slots and its
+ * output rows are zeros. */
 int ptts_b200_attend_scored(ptts_b200_kv* kv, int layer, const void* q, const void* k, const void* v,
                             int in_dtype, int num_kv_heads, const int32_t* streams_host,
                             const int32_t* rows_host, int n_seq, float max_period,

@@ -41,3 +41,78 @@ def test_first_token_calls_on_a_side_stream_beside_a_busy_default_stream(ptts, c
     all43.kv.check()
     for out, want, bound in got:
         compare(out, want, bound)
+
+
+CALLS = {  # name: (cached, rows, tree)
+    "tokens": ([5000, 40, 0, 300], [1, 1, 1, 1], False),
+    "rows": ([5000, 40, 0, 300], [9, 2, 70, 64], False),
+    "prompts": ([500, 40, 0, 300], [200, 129, 300, 7], False),
+    "trees": ([5000, 40, 0, 300], [9, 64, 33, 1], True),
+}
+
+
+def attend(ptts, b, tree, **kw):
+    args = (b.kv, 0, b.q, b.k, b.v, b.streams, b.rows)
+    return ptts.attend_tree(*args, b.parents_dev, **kw) if tree else ptts.attend_scored(*args, **kw)
+
+
+def device_lengths(b, lengths):
+    """The lengths as a caller's replayed graph would leave them: the device's alone."""
+    import torch
+    torch.cuda.synchronize()
+    b.kv.tensors(0)[2][torch.from_numpy(b.streams).long().to(b.cuda)] = torch.tensor(lengths, dtype=torch.int32, device=b.cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("host", [0, 3])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("kind", list(CALLS))
+def test_rows_go_by_the_devices_lengths(ptts, cuda, kind, dtype, host):
+    """Lengths that moved on the device alone: the rows' places, spans and work are the device's."""
+    cached, rows, tree = CALLS[kind]
+    b = Batch(ptts, cuda, cached, rows, dtype=dtype, tree=tree, seed=31)
+    b.kv.set_lengths(b.streams, [host] * len(cached))
+    device_lengths(b, cached)
+    out = attend(ptts, b, tree, softcap=20.0, slopes=b.slopes)
+    b.kv.check()
+    compare(out, *b.want(softcap=20.0, slopes=b.slopes, tree=tree, half_p=PAIR_HALF))
+    b.check_rows(tree=tree)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("spans", [False, True])
+@pytest.mark.parametrize("past", ["one", "most", "before", "least"])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("kind", list(CALLS))
+def test_a_device_length_that_does_not_fit_refuses_its_sequence(ptts, cuda, kind, dtype, past, spans):
+    """The last stream of the cache and another one: nothing written, zeros, the error word; the rest as ever."""
+    import torch
+    cached, rows, tree = CALLS[kind]
+    b = Batch(ptts, cuda, cached, rows, dtype=dtype, tree=tree, seed=32, spare=0)
+    refused = [int(np.argmax(b.streams)), (int(np.argmax(b.streams)) + 1) % 4]  # sequences
+    lengths = list(cached)
+    for i in refused:
+        lengths[i] = {"one": b.capacity - rows[i] + 1, "most": 2 ** 31 - 1, "before": -1, "least": -2 ** 31}[past]
+    device_lengths(b, lengths)
+    before = [t.clone() for t in b.kv.tensors(0)[:2]]
+    first = b.dev(np.zeros(sum(rows), np.int32)) if spans else None
+    last = b.dev(np.full(sum(rows), 2 ** 31 - 1, np.int32)) if spans and not tree else None
+    out = attend(ptts, b, tree, first=first, **({} if tree else {"last": last}))
+    with pytest.raises(ptts.PttsError) as e:
+        b.kv.check()
+    assert e.value.code == ptts.ERR_DEVICE and "capacity" in e.value.msg and "bounds" not in e.value.msg
+    offsets = np.r_[0, np.cumsum(rows)]
+    keep = np.ones(sum(rows), bool)
+    for i in refused:
+        keep[offsets[i]:offsets[i + 1]] = False
+        for t, old in zip(b.kv.tensors(0)[:2], before):
+            st = int(b.streams[i])
+            raw = torch.int16 if dtype == "bf16" else torch.int32
+            assert torch.equal(t[st].contiguous().view(raw), old[st].contiguous().view(raw))
+    assert (out[torch.from_numpy(~keep)] == 0).all()
+    for t in b.kv.tensors(0)[:2]:
+        t.copy_(torch.nan_to_num(t))  # so that the oracle has numbers in the refused streams
+    kw = {} if last is None else {"first": first.cpu().numpy(), "last": last.cpu().numpy().astype(np.int64)}
+    want, bound = b.want(tree=tree, half_p=PAIR_HALF, **kw)
+    keep = torch.from_numpy(keep)
+    compare(out[keep], want[keep], bound[keep])

@@ -662,7 +662,9 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
             most = std::max(most, blocks.back().y);
         }
     const int n_few = (int)blocks.size();
-    if (n_few) grid = score_rows_grid(out_bf16, kv->heads, sms);
+    int most_keys = 0;
+    for (int i = 0; i < n_seq; ++i) most_keys = std::max(most_keys, kv->h_len[streams_host[i]] + rows_host[i]);
+    if (n_few) grid = score_rows_grid(out_bf16, kv->heads, sms, (long long)n_few * most_keys, n_few);
     if (!tokens && !cache_bf16)
         for (int i = 0; i < n_seq; ++i)
             for (int r = offsets[i]; r < offsets[i + 1]; r += kScoreF32Rows)
@@ -679,12 +681,9 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
     const size_t blocks_at = append_tiles(packed, blocks);
     const bool inlined = packed.size() <= (size_t)kScoreInline;
     const int n_units = few ? n_few : tokens ? n_rows : 0;
-    int most_keys = 0;
-    for (int i = 0; i < n_seq; ++i) most_keys = std::max(most_keys, kv->h_len[streams_host[i]] + rows_host[i]);
-    const long long few_keys = (long long)n_few * most_keys;  // at most
     const int splits = !tokens && !cache_bf16 ? score_f32_splits(n_tiles, kv->heads, most_keys, sms) : 1;
     const size_t part_floats = tokens ? decode_part_floats(n_rows, grid) * kv->groups()
-                               : few  ? score_rows_part_floats(kv->heads, grid, few_keys, n_few, most)
+                               : few  ? score_rows_part_floats(kv->heads, grid, most)
                                       : splits > 1 ? (size_t)kPartStride * splits * kv->heads * n_rows : 0;
     // The scratch, cut into 256-byte aligned parts.
     size_t bytes = 0;

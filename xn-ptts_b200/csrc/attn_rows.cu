@@ -678,15 +678,12 @@ void launch_rules(const ScoreRowsArgs& a, const CUtensorMap* m, int grid, cudaSt
 
 }  // namespace
 
-int score_rows_grid(bool out_bf16, int heads, int sms) {
+int score_rows_grid(bool out_bf16, int heads, int sms, long long keys, int blocks) {
     const int slabs = heads / (out_bf16 ? 2 : 1);
-    return sms / slabs > 1 ? sms / slabs : 1;
+    return score_ctas(keys * score_key_cost(kTreeNodes) + (long long)blocks * kScoreBlockCost, sms / slabs > 1 ? sms / slabs : 1);
 }
 
-size_t score_rows_part_floats(int heads, int grid, long long keys, int blocks, int most_rows) {
-    const long long ctas = score_ctas(keys * score_key_cost(kTreeNodes) + (long long)blocks * kScoreBlockCost, grid);  // at most
-    return (size_t)2 * ctas * heads * most_rows * kPartStride;
-}
+size_t score_rows_part_floats(int heads, int grid, int most_rows) { return (size_t)2 * grid * heads * most_rows * kPartStride; }
 
 bool launch_score_rows(const ScoreRowsArgs& a, int grid, cudaStream_t s) {
     CUtensorMap m[4];

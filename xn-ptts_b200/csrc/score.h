@@ -144,9 +144,10 @@ struct ScoreRowsArgs {
     float* part;          // score_rows_part_floats
     uint32_t* err;
 };
-int score_rows_grid(bool out_bf16, int heads, int sms);  // CTAs along the keys (the plan's grid)
-// For `keys` keys of all blocks (an upper bound).
-size_t score_rows_part_floats(int heads, int grid, long long keys, int blocks, int most_rows);
+// CTAs along the keys (the plan's grid, and the most that the kernels use whatever the device's lengths
+// are), for `keys` keys of all blocks (an upper bound).
+int score_rows_grid(bool out_bf16, int heads, int sms, long long keys, int blocks);
+size_t score_rows_part_floats(int heads, int grid, int most_rows);
 bool launch_score_rows(const ScoreRowsArgs& a, int grid, cudaStream_t s);
 
 // Prompts on tcgen05, bf16 caches (attn_score_prompt.cu): tiles (first row, rows) of up to 128

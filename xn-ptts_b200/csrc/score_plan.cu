@@ -43,6 +43,12 @@ __device__ __forceinline__ int seq_of_warp(const ScorePlanArgs& a, const int32_t
     return lo;
 }
 
+// Whether a sequence of `rows` rows fits behind the device's length `base`. The host has checked its own
+// lengths; the device's can be others (a caller's graph that advances, a caller that writes them).
+__device__ __forceinline__ bool fits(const ScorePlanArgs& a, int base, int rows) {
+    return base >= 0 && base <= a.capacity - rows;
+}
+
 // Row r's visible slots, from the caller's spans clamped to the filled slots; an empty span is
 // 0..-1 whatever the caller wrote.
 __device__ __forceinline__ void row_span(const ScorePlanArgs& a, int r, int base, int row0, int rows, int& lo, int& hi) {
@@ -53,7 +59,7 @@ __device__ __forceinline__ void row_span(const ScorePlanArgs& a, int r, int base
 }
 
 // CTA 0: the units' key counts, end to end. Every unit has at least one key, so that a CTA visits
-// it and writes its rows even where they see nothing.
+// it and writes its rows even where they see nothing; a sequence that does not fit has that one, in slot 0.
 __device__ __forceinline__ void plan_units(const ScorePlanArgs& a, const int32_t* list) {
     __shared__ int warp_tot[kPlanWarps];
     __shared__ int carry;
@@ -73,8 +79,8 @@ __device__ __forceinline__ void plan_units(const ScorePlanArgs& a, const int32_t
             const int base = a.lengths[streams[sq]], rows = offsets[sq + 1] - row0;
             int lo = 0x7fffffff, hi = -1;
             for (int i = lane; i < b.y; i += 32) {
-                int x, y;
-                row_span(a, b.x + i, base, row0, rows, x, y);
+                int x = 0, y = -1;
+                if (fits(a, base, rows)) row_span(a, b.x + i, base, row0, rows, x, y);
                 if (x <= y) lo = min(lo, x), hi = max(hi, y);
             }
 #pragma unroll
@@ -99,8 +105,8 @@ __device__ __forceinline__ void plan_units(const ScorePlanArgs& a, const int32_t
                 const int2 b = unit(u);
                 const int sq = seq_of(a, offsets, b.x), row0 = offsets[sq];
                 const int base = a.lengths[streams[sq]], rows = offsets[sq + 1] - row0;
-                int lo, hi;
-                row_span(a, b.x + b.y - 1, base, row0, rows, lo, hi);  // without spans the last row sees the most
+                int lo = 0, hi = -1;
+                if (fits(a, base, rows)) row_span(a, b.x + b.y - 1, base, row0, rows, lo, hi);  // without spans the last row sees the most
                 a.unit_lo[u] = lo;
                 v = max(hi - lo + 1, 1);
             }
@@ -174,7 +180,7 @@ __device__ __forceinline__ void plan(const ScorePlanArgs& a, const int32_t* list
     const bool known = sid >= 0 && sid < a.num_streams;
     const int base = known ? a.lengths[sid] : 0;
     const int node = r - row0, slot = base + node;
-    bool good = known && base >= 0 && slot < a.capacity;
+    bool good = known && fits(a, base, rows);  // the whole sequence: its rows see each other's slots
     if (!good && lane == 0) set_error(a.err, known ? DEV_ERR_CAPACITY : DEV_ERR_BOUNDS);
     int pos = slot, lo = 0, hi = -1;
     if (good) row_span(a, r, base, row0, rows, lo, hi);
