@@ -53,7 +53,7 @@ extern "C" {
 
 /* Bits of the device-side error word (ptts_b200_kv_check reads the kv's own word;
  * ptts_b200_attend_decode_noalloc ORs them into the caller's). */
-#define PTTS_B200_DEVERR_BOUNDS 1u    /* an index outside its range (streams, parents) */
+#define PTTS_B200_DEVERR_BOUNDS 1u    /* an index outside its range (streams, parents, an accepted path) */
 #define PTTS_B200_DEVERR_CAPACITY 2u  /* a row's position outside its stream's slots */
 #define PTTS_B200_DEVERR_TIMEOUT 4u   /* a bounded wait inside a kernel gave up */
 #define PTTS_B200_DEVERR_DUPLICATE 8u /* a stream named by two rows of one decode call */
@@ -269,7 +269,9 @@ int ptts_b200_attend_tree(ptts_b200_kv* kv, int layer, const void* q, const void
  * stream's after another's, rising: a root, a child of it, ...) move to the slots behind the
  * cached rows in every layer, and the stream's length grows by their number. A count may be 0.
  * Refused as a whole, before anything changes: a stream named twice, nodes that do not rise within
- * 0..63, a node outside the capacity, rings and windowed streams, capture in a CUDA graph. */
+ * 0..63, a node outside the capacity, rings and windowed streams, capture in a CUDA graph. A stream whose
+ * length on the device is not the host's (see ptts_b200_attend_scored) is refused on the device
+ * (PTTS_B200_DEVERR_BOUNDS) and keeps its rows and its length there; ptts_b200_kv_set_lengths sets both. */
 int ptts_b200_kv_accept(ptts_b200_kv* kv, const int32_t* streams_host, const int32_t* counts_host,
                         const int32_t* nodes_host, int n, void* cuda_stream);
 

@@ -116,3 +116,40 @@ def test_a_device_length_that_does_not_fit_refuses_its_sequence(ptts, cuda, kind
     want, bound = b.want(tree=tree, half_p=PAIR_HALF, **kw)
     keep = torch.from_numpy(keep)
     compare(out[keep], want[keep], bound[keep])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("by", [-1, 1, 2])
+@pytest.mark.parametrize("times", [1, 60])
+def test_accept_refuses_a_stream_whose_device_length_is_another(ptts, cuda, by, times):
+    """Also where the device is ahead by just the path's length. `times` 60: a list too long for the parameters."""
+    import torch
+    n = 4 * times
+    b = Batch(ptts, cuda, [10 + i % 7 for i in range(n)], [20] * n, layers=2, seed=33)
+    for l in range(2):
+        for t in b.kv.tensors(l)[:2]:
+            t.copy_(torch.randn(t.shape, device=cuda))
+    wrong = [i for i in range(n) if i % 4 == 1]
+    lengths = np.array(b.cached)
+    lengths[wrong] += by
+    device_lengths(b, lengths)
+    want = [[t.clone() for t in b.kv.tensors(l)[:2]] for l in range(2)]
+    for i, (st, L) in enumerate(zip(b.streams, b.cached)):
+        for layer in want if i not in wrong else []:
+            for t in layer:
+                t[int(st), int(L):int(L) + 2] = t[int(st), [int(L) + 3, int(L) + 7]]
+    b.kv.accept(b.streams, [[3, 7]] * n)
+    with pytest.raises(ptts.PttsError) as e:
+        b.kv.check()
+    assert e.value.code == ptts.ERR_DEVICE and "bounds" in e.value.msg
+    for l in range(2):
+        for t, w in zip(b.kv.tensors(l)[:2], want[l]):
+            assert torch.equal(t, w)
+    lengths[[i for i in range(n) if i not in wrong]] += 2
+    got = b.kv.tensors(0)[2].cpu().numpy()[b.streams]
+    np.testing.assert_array_equal(got, lengths)
+    # Lengths set on both sides: the next acceptance goes through (the arrivals were left at zero).
+    b.kv.set_lengths(b.streams, b.cached)
+    b.kv.accept(b.streams, [[0]] * n)
+    b.kv.check()
+    np.testing.assert_array_equal(b.kv.tensors(0)[2].cpu().numpy()[b.streams], b.cached + 1)

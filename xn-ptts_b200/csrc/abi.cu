@@ -180,6 +180,7 @@ struct ptts_b200_kv {
     std::vector<int32_t> h_window;
     // scratch of the attention op
     DevBuf seq_stream, row_offsets, row_stream, row_pos, prefix, part, q_rot, counters;
+    DevBuf arrived;  // [streams] zeros, of the acceptance (AcceptArgs)
     // scratch of the scored and tree attention, one allocation for a call's lists, plan, q and records
     DevBuf score;
     Staging staging;
@@ -1432,6 +1433,7 @@ int ptts_b200_kv_create(int device, int num_layers, int num_streams, int capacit
         kv->h_ring_valid.assign((size_t)num_streams * capacity, 0);
         CK(cudaMemset(kv->window.need(sizeof(int32_t) * num_streams), 0, sizeof(int32_t) * num_streams));
         kv->h_window.assign(num_streams, 0);
+        CK(cudaMemset(kv->arrived.need(sizeof(int32_t) * num_streams), 0, sizeof(int32_t) * num_streams));
         CK(cudaDeviceSynchronize());
         *out = kv.release();
     });
@@ -1794,6 +1796,7 @@ int ptts_b200_kv_accept(ptts_b200_kv* kv, const int32_t* streams_host, const int
         a.capacity = kv->capacity;
         a.n = n;
         a.lengths = kv->len.as<int32_t>();
+        a.arrived = kv->arrived.as<int32_t>();
         a.err = kv->err.as<uint32_t>();
         if (list.size() <= (size_t)kAcceptInline) {
             AcceptInline in;

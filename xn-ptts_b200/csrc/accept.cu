@@ -20,11 +20,24 @@ __device__ __forceinline__ void accept(const AcceptArgs& a, const int32_t* list)
     const int from = offsets[i], count = offsets[i + 1] - from;
     const int32_t* node = offsets + a.n + 1 + from;
     const bool first = blockIdx.y == 0 && threadIdx.x == 0;
-    if (sid < 0 || sid >= a.streams || len < 0 || (count > 0 && len + node[count - 1] >= a.capacity)) {
-        if (first) set_error(a.err, sid < 0 || sid >= a.streams ? DEV_ERR_BOUNDS : DEV_ERR_CAPACITY);
+    // The nodes lie behind the device's length: where that is not the host's, the path is refused.
+    if (sid < 0 || sid >= a.streams || len < 0 || *const_cast<volatile int32_t*>(a.lengths + sid) != len) {
+        if (first) set_error(a.err, DEV_ERR_BOUNDS);
         return;
     }
-    if (first) a.lengths[sid] = len + count;
+    if (count > 0 && len + node[count - 1] >= a.capacity) {
+        if (first) set_error(a.err, DEV_ERR_CAPACITY);
+        return;
+    }
+    // All of the stream's CTAs come here or none: the one that finds the others' reads done writes the length.
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        if (atomicAdd(a.arrived + sid, 1) == (int)gridDim.y - 1) {
+            a.lengths[sid] = len + count;
+            a.arrived[sid] = 0;
+        }
+    }
     const int c = blockIdx.y * blockDim.x + threadIdx.x;
     if (c >= 2 * a.blocks * a.row_vec) return;
     const int b = c / a.row_vec;

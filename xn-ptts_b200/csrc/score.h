@@ -170,8 +170,8 @@ struct ScorePromptArgs {
 bool launch_score_prompt(const ScorePromptArgs& a, cudaStream_t s);
 
 // Acceptance: per stream the accepted nodes' rows move from slot len + node[j] to len + j, in
-// every layer and head group, and the length becomes len + their number. Nodes rise, so
-// node[j] >= j. The lists are one array of int32 (host or device): streams [n], lengths before
+// every layer and head group, and the length becomes len + their number. A stream whose length on the
+// device is not `len` is refused there (DEV_ERR_BOUNDS) and stays as it is. Nodes rise, so node[j] >= j. The lists are one array of int32 (host or device): streams [n], lengths before
 // [n], offsets into the nodes [n + 1], nodes.
 constexpr int kAcceptInline = 512;
 struct AcceptInline {  // a short list rides in the launch's parameters
@@ -187,6 +187,7 @@ struct AcceptArgs {
     int streams, capacity;
     int n;
     int32_t* lengths;
+    int32_t* arrived;  // [streams] zeros: CTAs of a stream that have read its length
     uint32_t* err;
 };
 void launch_accept(const AcceptArgs& a, const int32_t* list_dev, cudaStream_t s);
