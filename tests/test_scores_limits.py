@@ -153,3 +153,20 @@ def test_accept_refuses_a_stream_whose_device_length_is_another(ptts, cuda, by, 
     b.kv.accept(b.streams, [[0]] * n)
     b.kv.check()
     np.testing.assert_array_equal(b.kv.tensors(0)[2].cpu().numpy()[b.streams], b.cached + 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("cached,last", [(20, 9), (6000, 4000), (40000, 39000)])
+def test_a_cut_row_far_below_every_score_is_joined(ptts, cuda, dtype, cached, last):
+    """Slopes that put every key a row sees below -10^31: the nearest has all the weight, exactly, whether the
+    row is one CTA's or cut among many. (Distances differ by 1e28 after f32's rounding of 2^-24 x 6e32.)"""
+    import torch
+    b = Batch(ptts, cuda, [cached, cached], [1, 1], dtype=dtype, seed=41)
+    last = b.dev(np.full(2, last, np.int32))
+    out = ptts.attend_scored(b.kv, 0, b.q, b.k, b.v, b.streams, b.rows, last=last, max_period=0.0,
+                             slopes=torch.full((8,), 1e28, device=cuda))
+    b.kv.check()
+    vt = b.kv.tensors(0)[1]
+    want = torch.stack([vt[int(st), int(last[0])].float().reshape(512) for st in b.streams])
+    assert torch.equal(out, want)

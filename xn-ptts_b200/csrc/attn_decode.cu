@@ -167,7 +167,7 @@ __device__ __forceinline__ void store_out(const DecodeArgs& a, long long at, int
 // Merge the partial records of stream b, head h, written by CTAs c0..c1 (one warp; lane owns
 // dims 2*lane, 2*lane+1). Records of other CTAs are read past L1.
 __device__ __forceinline__ void merge_head(const DecodeArgs& a, int b, int h, int c0, int c1, int lane) {
-    float mx = -1e30f;
+    float mx = kScoreLow;  // below every record's maximum, a scored row's (kLow) too
     for (int c = c0; c <= c1; ++c)
         mx = fmaxf(mx, __ldcg(a.part + ((long long)(b + c) * kHeads + h) * kPartStride + 64));
     float n0 = 0.f, n1 = 0.f, den = 0.f;
