@@ -170,3 +170,20 @@ def test_a_cut_row_far_below_every_score_is_joined(ptts, cuda, dtype, cached, la
     vt = b.kv.tensors(0)[1]
     want = torch.stack([vt[int(st), int(last[0])].float().reshape(512) for st in b.streams])
     assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_an_infinite_value_in_a_tokens_last_key_is_infinite(ptts, cuda, dtype):
+    """A token sees itself: an infinity in its value is one in its output, at every place in a chunk of keys."""
+    import torch
+    cached = list(range(0, 70)) + [700, 2501]
+    b = Batch(ptts, cuda, cached, [1] * len(cached), dtype=dtype, seed=42)
+    args = (b.kv, 0, b.q, b.k, b.v, b.streams, b.rows)
+    clean = ptts.attend_scored(*args, softcap=30.0).reshape(-1, 8, 64).clone()
+    b.v[:, :, 3], b.v[:, :, 60] = float("inf"), -float("inf")
+    out = ptts.attend_scored(*args, softcap=30.0).reshape(-1, 8, 64)
+    b.kv.check()
+    rest = [d for d in range(64) if d not in (3, 60)]
+    assert torch.equal(out[..., rest], clean[..., rest])
+    assert (out[..., 3] == float("inf")).all() and (out[..., 60] == -float("inf")).all()

@@ -433,8 +433,10 @@ __global__ void __launch_bounds__(kThreads, 1) decode_attn_kernel(DecodeArgs a) 
                 float v[8];
                 widen(rv, v);
                 const float w = __shfl_sync(0xffffffffu, e, (lane & 24) | i);
+                if (r < n) {  // the row read in place of one past the end adds nothing, not even 0 x inf
 #pragma unroll
-                for (int x = 0; x < 8; ++x) acc[x] = fmaf(w, v[x], acc[x]);
+                    for (int x = 0; x < 8; ++x) acc[x] = fmaf(w, v[x], acc[x]);
+                }
             }
         } else {
 #pragma unroll
