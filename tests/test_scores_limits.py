@@ -7,7 +7,7 @@ import copy
 import numpy as np
 import pytest
 
-from test_scores import PAIR_HALF, Batch, compare
+from test_scores import PAIR_HALF, Batch, compare, lineages
 
 
 def of_streams(b, n):
@@ -187,3 +187,53 @@ def test_an_infinite_value_in_a_tokens_last_key_is_infinite(ptts, cuda, dtype):
     rest = [d for d in range(64) if d not in (3, 60)]
     assert torch.equal(out[..., rest], clean[..., rest])
     assert (out[..., 3] == float("inf")).all() and (out[..., 60] == -float("inf")).all()
+
+
+class Far:
+    """One stream whose cached rows end past position 2^24, of which the last 300 and the call's `rows` hold
+    numbers; the oracle reads those alone (no rotation, so only differences of positions count)."""
+
+    def __init__(self, ptts, cuda, rows, dtype, tree):
+        import torch
+        self.start = 16_800_001 - 300
+        self.kv = ptts.KvState(1, 1, 16_800_001 + rows, dtype=dtype)
+        self.kv.set_lengths([0], [16_800_001])
+        kt, vt, _ = self.kv.tensors(0)
+        for t in (kt, vt):
+            t[0, self.start:] = torch.randn(300 + rows, 8, 64, device=cuda).to(t.dtype)
+        b = self.b = Batch(ptts, cuda, [300], [rows], dtype=dtype, tree=tree, spare=0, seed=43)
+        b.kv.close()
+        b.kv = self
+        b.streams = np.zeros(1, np.int32)
+
+    def tensors(self, layer):
+        kt, vt, lt = self.kv.tensors(layer)
+        return kt[:, self.start:], vt[:, self.start:], lt
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["rows", "trees", "prompts", "tokens", "f32 rows", "f32 trees"])
+def test_a_distance_bias_past_2_24_positions(ptts, cuda, kind):
+    """Distances of near keys are whole numbers however far both are from 0 (an f32 position past 2^24 is
+    even). Bounds as in test_scores.py."""
+    import torch
+    tree, dtype = kind.endswith("trees"), "f32" if kind.startswith("f32") else "bf16"
+    rows = {"tokens": 1, "prompts": 1500}.get(kind, 40)  # 1500: too many blocks for the rows kernel
+    far = Far(ptts, cuda, rows, dtype, tree)
+    b = far.b
+    pos = 300 + (np.array(lineages(b.parents[0])[0]) if tree else np.arange(rows))
+    first = (pos - 100).astype(np.int32)
+    slopes = torch.tensor([0.5, 0.25, 1.0, 0.125, 0.75, 0.5, 2.0, 0.0625], device=cuda)
+    for softcap in (0.0, 30.0):
+        for out_dtype in ("bf16", "f32"):
+            args = (far.kv, 0, b.q, b.k, b.v, [0], [rows])
+            rules = dict(softcap=softcap, slopes=slopes, max_period=0.0)
+            at = b.dev(first + np.int32(far.start))
+            if tree:
+                out = ptts.attend_tree(*args, b.parents_dev, first=at, out_dtype=out_dtype, **rules)
+            else:
+                out = ptts.attend_scored(*args, first=at, out_dtype=out_dtype, **rules)
+            half_out, half_p = b.halves(out_dtype)
+            compare(out, *b.want(first=first, tree=tree, half_out=half_out, half_p=half_p, **rules))
+    far.kv.check()
+    far.kv.close()

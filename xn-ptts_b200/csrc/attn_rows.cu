@@ -69,7 +69,7 @@ struct Smem {
 };
 // A head's rows of the block at hand.
 struct HeadRows {
-    float m[NR], shift[NR], scale[NR], pos[NR], sum[NR];
+    float m[NR], shift[NR], scale[NR], pos[NR], sum[NR];  // pos: less the first row's
     int lo[NR], hi[NR], top[NR], has[NR];  // has: the row has a maximum (or sees nothing)
     unsigned long long lineage[NR];
     int bad;
@@ -223,13 +223,16 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
         while (!idle && w.next()) {
             // The block's rows.
             const int base_slot = a.rows.lineage ? a.rows.base[w.row0] : 0x7fffffff;
+            // Positions for the bias count from the block's first row: the block's rows are near it, so the
+            // distances of near keys are exact in f32 wherever the block is (positions past 2^24 are not).
+            const int origin = a.rows.pos[w.row0];
             if (key < NR) {
                 const bool there = key < w.nrows;
                 const int row = w.row0 + (there ? key : 0);
                 const int lo = there ? a.rows.lo[row] : 0, hi = there ? a.rows.hi[row] : -1, pos = a.rows.pos[row];
                 R->lo[key] = lo;
                 R->hi[key] = hi;
-                R->pos[key] = (float)pos;
+                R->pos[key] = (float)(pos - origin);
                 R->lineage[key] = there && a.rows.lineage ? a.rows.lineage[row] : 0;
                 // BOUNDED: exp2 against the row's greatest bias (a node sees positions lo .. its own). Else the
                 // row's first scores set m.
@@ -280,7 +283,7 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
                         }
                     }
                 }
-                float at = (float)slot;  // the key's position
+                float at = (float)(slot - origin);  // the key's position
                 if (biased && slot >= base_slot) at = R->pos[min(slot - base_slot, NR - 1)];
                 ok = ok && __all_sync(0xffffffffu, mbar_wait(&b->sfull, i & 1));
                 float s[NR];

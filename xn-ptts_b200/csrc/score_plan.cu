@@ -211,7 +211,7 @@ __device__ __forceinline__ void plan(const ScorePlanArgs& a, const int32_t* list
     }
     if (lane == 0) {
         a.rows.stream[r] = good ? sid : -1;
-        a.rows.pos[r] = pos;
+        a.rows.pos[r] = good ? pos : 0;
         a.rows.lo[r] = lo;
         a.rows.hi[r] = hi;
         if (a.parents) {
