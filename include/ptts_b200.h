@@ -257,8 +257,9 @@ int ptts_b200_attend_scored(ptts_b200_kv* kv, int layer, const void* q, const vo
  * itself; it sits at position length + depth (rotation and bias), and its k and v are written to
  * slot length + index. scores->first limits both to positions from it on; scores->last must be
  * NULL. A parent out of range refuses its sequence on the device (PTTS_B200_DEVERR_BOUNDS in
- * ptts_b200_kv_check): nothing is written to its slots and its output rows are zeros. Otherwise
- * as ptts_b200_attend_scored. */
+ * ptts_b200_kv_check): nothing is written to its slots and its output rows are zeros. On bf16 caches
+ * n_seq * (7 * capacity + 2560) is below 2^31 (PTTS_B200_ERR_UNSUPPORTED; 800,000 trees on streams of 17
+ * slots). Otherwise as ptts_b200_attend_scored. */
 int ptts_b200_attend_tree(ptts_b200_kv* kv, int layer, const void* q, const void* k, const void* v,
                           int in_dtype, int num_kv_heads, const int32_t* streams_host,
                           const int32_t* rows_host, int n_seq, const int32_t* parents, float max_period,

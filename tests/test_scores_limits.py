@@ -237,3 +237,27 @@ def test_a_distance_bias_past_2_24_positions(ptts, cuda, kind):
             compare(out, *b.want(first=first, tree=tree, half_out=half_out, half_p=half_p, **rules))
     far.kv.check()
     far.kv.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_hundreds_of_thousands_of_trees(ptts, cuda, dtype):
+    """One-node trees on empty streams: each node's value, exactly. More than the plan's sum of costs can count
+    is refused before anything changes (bf16; the f32 kernel counts no costs)."""
+    import torch
+    n = 900_000
+    kv = ptts.KvState(1, n, 2, dtype=dtype)
+    x = torch.randn(n, 8, 64, device=cuda).to(torch.bfloat16 if dtype == "bf16" else torch.float32)
+    roots = torch.full((n,), -1, dtype=torch.int32, device=cuda)
+    streams, one = np.arange(n, dtype=np.int32), np.ones(n, np.int32)
+    out = torch.full((n, 512), 7.0, device=cuda)
+    if dtype == "bf16":
+        with pytest.raises(ptts.PttsError) as e:
+            ptts.attend_tree(kv, 0, x, x, x, streams, one, roots, out=out)
+        assert e.value.code == ptts.ERR_UNSUPPORTED
+        assert (out == 7.0).all() and not kv.tensors(0)[1].any()
+        n = 800_000
+    ptts.attend_tree(kv, 0, x[:n], x[:n], x[:n], streams[:n], one[:n], roots[:n], out=out[:n])
+    kv.check()
+    assert torch.equal(out[:n].view(n, 8, 64), x[:n].float()) and torch.equal(kv.tensors(0)[1][:n, 0], x[:n])
+    kv.close()

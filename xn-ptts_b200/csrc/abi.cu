@@ -580,6 +580,12 @@ void refuse_capture(cudaStream_t s, const char* what) {
         fail(PTTS_B200_ERR_STATE, std::string(what) + " plans from the host's lengths: it cannot be captured in a CUDA graph");
 }
 
+// Whether `blocks` blocks of rows, each of which can see a whole stream, keep the plan's sum of costs within
+// its 32 bits.
+bool block_costs_fit(const ptts_b200_kv* kv, double blocks) {
+    return blocks * ((double)kv->capacity * score_key_cost(kTreeNodes) + kScoreBlockCost) < 2147483648.0;
+}
+
 // Which sequences of a call on a bf16 cache run on the rows kernel (blocks of 64 rows split over the keys)
 // rather than in the prompt kernel's tiles of 128 rows. Trees: all. Others by estimated times (us on one
 // B200, 8 heads, measured over 1-64 sequences of 16-512 rows on 0-30000 keys): a tile takes 0.0113 a key
@@ -593,16 +599,16 @@ std::vector<char> few_row_sequences(const ptts_b200_kv* kv, const int32_t* strea
     std::vector<char> few(n_seq, tree);
     if (tree) return few;
     const double per_tile = 0.0113, full = 0.000305 * kv->groups(), per_block = 0.0005 * kv->groups(), start = 14.0;
-    double all = 0.0, blocks = start, longest = 0.0, block_keys = 0.0;
+    double all = 0.0, blocks = start, longest = 0.0, n_blocks = 0.0;
     auto keys = [&](int i) { return (double)kv->h_len[streams[i]] + rows[i]; };
     for (int i = 0; i < n_seq; ++i) all += full * ((rows[i] + 127) / 128) * keys(i);
     for (int i = 0; i < n_seq; ++i)
         if ((few[i] = per_tile * keys(i) > all + start)) {
             blocks += per_block * ((rows[i] + kTreeNodes - 1) / kTreeNodes) * keys(i);
-            block_keys += (rows[i] + kTreeNodes - 1) / kTreeNodes * keys(i);
+            n_blocks += (rows[i] + kTreeNodes - 1) / kTreeNodes;
             longest = std::max(longest, per_tile * keys(i));
         }
-    if (blocks > longest || block_keys > 2e8) few.assign(n_seq, 0);
+    if (blocks > longest || !block_costs_fit(kv, n_blocks)) few.assign(n_seq, 0);
     return few;
 }
 
@@ -643,6 +649,9 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
             if (rows_host[i] > kTreeNodes)
                 fail(PTTS_B200_ERR_UNSUPPORTED, "a tree has at most " + std::to_string(kTreeNodes) + " nodes, not " +
                                                     std::to_string(rows_host[i]));
+        if (kv->dtype == PTTS_B200_BF16 && !block_costs_fit(kv, n_seq))
+            fail(PTTS_B200_ERR_UNSUPPORTED, std::to_string(n_seq) + " trees in one call are too many on streams of " +
+                                                std::to_string(kv->capacity) + " slots");
     }
     DeviceScope scope(kv->device);
     refuse_capture(s, tree ? "ptts_b200_attend_tree" : "ptts_b200_attend_scored");
