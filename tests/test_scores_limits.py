@@ -261,3 +261,22 @@ def test_hundreds_of_thousands_of_trees(ptts, cuda, dtype):
     kv.check()
     assert torch.equal(out[:n].view(n, 8, 64), x[:n].float()) and torch.equal(kv.tensors(0)[1][:n, 0], x[:n])
     kv.close()
+
+
+class AnyStream:
+    cuda_stream = 0
+
+
+def refused_by_python(ptts, word, f, *a):
+    """Refused with `word` before the library is called (which would say that the handle is NULL)."""
+    with pytest.raises(ptts.PttsError) as e:
+        f(*a, stream=AnyStream)
+    assert e.value.code == ptts.ERR_ARG and word in e.value.msg, e.value
+
+
+def test_accept_takes_one_path_per_stream(ptts):
+    """Streams of another rank or number than the paths: the library would read past the counts. On no device."""
+    kv = object.__new__(ptts.KvState)
+    kv._h, kv.device = None, 0
+    for streams in (np.zeros((2, 2), np.int32), np.zeros((2, 1), np.int32), [[0, 1], [2, 3]], np.int32(3), [0], [0, 1, 2]):
+        refused_by_python(ptts, "one path per stream", kv.accept, streams, [[0], [0, 1]])

@@ -400,9 +400,10 @@ class KvState:
         """Keep the drafted nodes `nodes[i]` (rising indexes, a path of attend_tree's tree; may be
         empty) of stream `streams[i]`: their rows move behind the cached ones in every layer, and
         the stream grows by their number (ptts_b200_kv_accept)."""
-        if len(nodes) != len(streams):
+        st = _vec32(streams)
+        if st.ndim != 1 or st.size != len(nodes):
             raise PttsError(ERR_ARG, "one path per stream")
-        st, counts = _vec32(streams), np.fromiter(map(len, nodes), np.int32, len(nodes))
+        counts = np.fromiter(map(len, nodes), np.int32, len(nodes))
         try:  # node indexes are below 64: a batch of paths flattens fastest as bytes
             flat = np.frombuffer(bytes(chain.from_iterable(nodes)), np.uint8).astype(np.int32)
         except (ValueError, TypeError):  # an index that the library will refuse
