@@ -280,3 +280,14 @@ def test_accept_takes_one_path_per_stream(ptts):
     kv._h, kv.device = None, 0
     for streams in (np.zeros((2, 2), np.int32), np.zeros((2, 1), np.int32), [[0, 1], [2, 3]], np.int32(3), [0], [0, 1, 2]):
         refused_by_python(ptts, "one path per stream", kv.accept, streams, [[0], [0, 1]])
+
+
+def test_accepted_nodes_are_whole_numbers(ptts):
+    """An index that is not a whole number ([0, 1.5]) is no node; whole ones of any size get to the library, which
+    refuses those past 63 (and here says that the handle is NULL). On no device."""
+    kv = object.__new__(ptts.KvState)
+    kv._h, kv.device = None, 0
+    for path in ([0, 1.5], [0.0], np.array([0.0, 1.0]), ["a"], [None], [[0, 1]], np.zeros((2, 2), np.int64), 5):
+        refused_by_python(ptts, "node", kv.accept, [0], [path])
+    for path in ([0, 64], [0, 300], [-1], [0, 2 ** 40], [0, 2 ** 70], [1, 0], np.array([0, 7], np.int64)):
+        refused_by_python(ptts, "NULL", kv.accept, [0], [path])

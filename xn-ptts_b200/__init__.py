@@ -23,6 +23,7 @@ import ctypes
 import os
 from dataclasses import dataclass, field
 from itertools import chain
+from operator import index
 from typing import Optional, Sequence
 
 import numpy as np
@@ -403,11 +404,14 @@ class KvState:
         st = _vec32(streams)
         if st.ndim != 1 or st.size != len(nodes):
             raise PttsError(ERR_ARG, "one path per stream")
-        counts = np.fromiter(map(len, nodes), np.int32, len(nodes))
-        try:  # node indexes are below 64: a batch of paths flattens fastest as bytes
-            flat = np.frombuffer(bytes(chain.from_iterable(nodes)), np.uint8).astype(np.int32)
-        except (ValueError, TypeError):  # an index that the library will refuse
-            flat = _i32([x for path in nodes for x in path])
+        try:
+            counts = np.fromiter(map(len, nodes), np.int32, len(nodes))
+            try:  # node indexes are below 64: a batch of paths flattens fastest as bytes
+                flat = np.frombuffer(bytes(chain.from_iterable(nodes)), np.uint8).astype(np.int32)
+            except ValueError:  # an index past a byte, for the library to refuse
+                flat = np.array([min(max(index(x), -1), 64) for path in nodes for x in path], np.int32)
+        except TypeError:
+            raise PttsError(ERR_ARG, "a path is a list of whole node indexes") from None
         _check(lib().ptts_b200_kv_accept(self._h, st.ctypes.data, counts.ctypes.data, flat.ctypes.data, st.size,
                                          _stream_of(self.device, stream)))
 
