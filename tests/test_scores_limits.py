@@ -291,3 +291,16 @@ def test_accepted_nodes_are_whole_numbers(ptts):
         refused_by_python(ptts, "node", kv.accept, [0], [path])
     for path in ([0, 64], [0, 300], [-1], [0, 2 ** 40], [0, 2 ** 70], [1, 0], np.array([0, 7], np.int64)):
         refused_by_python(ptts, "NULL", kv.accept, [0], [path])
+
+
+@pytest.mark.gpu
+def test_a_call_that_finds_no_memory_fails_alone(ptts, cuda):
+    """The next call on another cache is not blamed for it."""
+    with pytest.raises(ptts.PttsError) as e:
+        ptts.KvState(1, 1, 400_000_000)  # 410 GB of keys
+    assert "out of memory" in e.value.msg
+    b = Batch(ptts, cuda, [5, 70], [1, 1], seed=44)
+    b.kv.set_lengths(b.streams, b.cached)
+    out = ptts.attend_scored(b.kv, 0, b.q, b.k, b.v, b.streams, b.rows)
+    b.kv.check()
+    compare(out, *b.want(half_p=PAIR_HALF))

@@ -26,10 +26,14 @@ struct Error {
 
 [[noreturn]] inline void fail(int code, const std::string& msg) { throw Error{code, msg}; }
 
+// A failed call's error is taken off the runtime's record too: the next launch's check would report it.
 #define CK(call)                                                                             \
     do {                                                                                     \
         cudaError_t e_ = (call);                                                             \
-        if (e_ != cudaSuccess) fail(PTTS_B200_ERR_CUDA, std::string(#call) + ": " + cudaGetErrorString(e_)); \
+        if (e_ != cudaSuccess) {                                                             \
+            cudaGetLastError();                                                              \
+            fail(PTTS_B200_ERR_CUDA, std::string(#call) + ": " + cudaGetErrorString(e_));    \
+        }                                                                                    \
     } while (0)
 
 template <class F>
