@@ -304,3 +304,63 @@ def test_a_call_that_finds_no_memory_fails_alone(ptts, cuda):
     out = ptts.attend_scored(b.kv, 0, b.q, b.k, b.v, b.streams, b.rows)
     b.kv.check()
     compare(out, *b.want(half_p=PAIR_HALF))
+
+
+GROW = r"""
+#include <cstdio>
+#include <cstdlib>
+#include "host.h"
+// A device of 100 bytes; a failed call's error stays until it is read.
+static size_t used = 0, sizes[64];
+static int allocations = 0;
+static cudaError_t last = cudaSuccess;
+extern "C" {
+cudaError_t cudaMalloc(void** p, size_t n) {
+    if (n > 100 - used) return last = cudaErrorMemoryAllocation;
+    used += n;
+    sizes[allocations] = n;
+    *p = &sizes[allocations++];
+    return cudaSuccess;
+}
+cudaError_t cudaFree(void* p) { used -= *static_cast<size_t*>(p); return cudaSuccess; }
+cudaError_t cudaGetLastError(void) { cudaError_t e = last; last = cudaSuccess; return e; }
+cudaError_t cudaDeviceSynchronize(void) { return cudaSuccess; }
+const char* cudaGetErrorString(cudaError_t) { return "out of memory"; }
+cudaError_t cudaMemsetAsync(void*, int, size_t, cudaStream_t) { return cudaSuccess; }
+}
+#define CHECK(x) do { if (!(x)) { std::printf("line %d: %s\n", __LINE__, #x); return 1; } } while (0)
+int main() {
+    ptts::host::DevBuf b;
+    CHECK(b.grow(3, 10) && b.bytes == 10 && allocations == 1);
+    CHECK(b.grow(10, 10) && allocations == 1);
+    CHECK(b.grow(11, 10) && b.bytes == 15 && used == 15);
+    CHECK(b.grow(80, 10) && b.bytes == 80 && used == 80);
+    CHECK(b.grow(90, 10) && b.bytes == 90 && used == 90);  // 120 are not there, 90 are
+    CHECK(last == cudaSuccess);
+    const int rc = ptts::host::guarded([&] { b.grow(101, 10); });
+    CHECK(rc == PTTS_B200_ERR_CUDA && last == cudaSuccess && b.p == nullptr && b.bytes == 0 && used == 0);
+    CHECK(b.grow(40, 10) && b.bytes == 40 && used == 40);
+    return 0;
+}
+"""
+
+
+def test_scratch_grows_to_what_is_needed_where_half_again_is_not_there(tmp_path):
+    """The buffer's growth against a device of 100 bytes, on the CPU."""
+    import os
+    import shutil
+    import subprocess
+    from conftest import ROOT
+    cxx = shutil.which("g++")
+    nvcc = next((c for c in ("/usr/local/cuda/bin/nvcc", shutil.which("nvcc")) if c and os.path.exists(c)), None)
+    if not cxx or not nvcc:
+        pytest.skip("no C++ compiler or no CUDA headers")
+    (tmp_path / "grow.cpp").write_text(GROW)
+    dirs = [os.path.join(ROOT, "include"), os.path.join(ROOT, "xn-ptts_b200", "csrc"),
+            os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc))), "include")]
+    exe = str(tmp_path / "grow")
+    r = subprocess.run([cxx, "-std=c++17", *[f"-I{d}" for d in dirs], str(tmp_path / "grow.cpp"), "-o", exe],
+                       capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout

@@ -707,9 +707,7 @@ void attend_with_scores(ptts_b200_kv* kv, int layer, const void* q, const void* 
                  at_lineage = part(tree ? sizeof(unsigned long long) * (size_t)n_rows : 0),
                  at_units = part(n_units ? sizeof(int32_t) * (2 * (size_t)n_units + 1 + grid) : 0),
                  at_part = part(sizeof(float) * part_floats);
-    // Grown by half at a time, from 1 MB: a cache that fills up row by row does not allocate row by row.
-    if (bytes > kv->score.bytes) kv->score.need(std::max({bytes, kv->score.bytes / 2 * 3, (size_t)1 << 20}));
-    char* ws = static_cast<char*>(kv->score.p);
+    char* ws = static_cast<char*>(kv->score.grow(bytes, (size_t)1 << 20));
     // The merge counters too come before the plan: a call that finds no memory has changed nothing.
     int* counters = !tokens ? nullptr
                             : static_cast<int*>(kv->counters.need_zeroed(sizeof(int) * decode_counter_ints(n_rows) * kv->groups(), s));

@@ -5,6 +5,7 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <cstring>
@@ -94,6 +95,20 @@ struct DevBuf {
         CK(cudaMalloc(&p, n));
         bytes = n;
         return p;
+    }
+    // Like need(), by half at a time from `least` on, so that a buffer that is asked for a little more at every
+    // call is not allocated at every call; where there is no room for that, what is needed.
+    void* grow(size_t n, size_t least) {
+        if (n <= bytes) return p;
+        const size_t more = std::max({n, bytes / 2 * 3, least});
+        release();
+        if (more > n && cudaMalloc(&p, more) == cudaSuccess) {
+            bytes = more;
+            return p;
+        }
+        cudaGetLastError();
+        p = nullptr;
+        return need(n);
     }
     // Free the memory (the buffer reads as empty again).
     void release() {
