@@ -364,3 +364,188 @@ def test_scratch_grows_to_what_is_needed_where_half_again_is_not_there(tmp_path)
     assert r.returncode == 0, r.stderr
     r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, r.stdout
+
+
+# ---- views, outputs, caps, refusals -------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("heads", [8, 16])
+def test_a_view_keeps_its_cache(ptts, cuda, heads, which):
+    import gc
+    import weakref
+    kv = ptts.KvState(2, 3, 5, num_heads=heads)
+    alive, view = weakref.ref(kv), kv.tensors(1)[which][1:]
+    del kv
+    gc.collect()
+    assert alive() is not None
+    view.fill_(3)
+    assert (view == 3).all()
+    del view
+    gc.collect()
+    assert alive() is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out_dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("kind", list(CALLS))
+def test_out_is_written_and_nothing_beside_it(ptts, cuda, kind, dtype, out_dtype):
+    import torch
+    cached, rows, tree = CALLS[kind]
+    a, b = (Batch(ptts, cuda, cached, rows, dtype=dtype, tree=tree, seed=34) for _ in range(2))
+    n = sum(rows)
+    room = torch.full((n + 4, 512), 7.0, device=cuda, dtype=torch.bfloat16 if out_dtype == "bf16" else torch.float32)
+    out = attend(ptts, a, tree, softcap=30.0, out=room[2:n + 2], out_dtype="f32")  # out's own type is what counts
+    want = attend(ptts, b, tree, softcap=30.0, out_dtype=out_dtype)
+    assert out.data_ptr() == room[2].data_ptr() and torch.equal(room[2:n + 2], want)
+    assert (room[:2] == 7).all() and (room[n + 2:] == 7).all()
+    a.kv.check(), b.kv.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [1.0, 30.0])
+@pytest.mark.parametrize("cap", [40.5, 50.0, 90.0, 128.0])
+@pytest.mark.parametrize("out_dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("kind", ["rows", "prompts", "trees"])
+def test_caps_above_40_without_a_bias(ptts, cuda, kind, out_dtype, cap, scale):
+    """Caps of the fast tanh that keep maxima, with scores far below the cap and past it. Bounds as in
+    test_scores.py: its score term charges the cap 2^-16, above the fast tanh's 3.6e-6 (2^-18)."""
+    cached, rows, tree = CALLS[kind]
+    b = Batch(ptts, cuda, cached, rows, tree=tree, seed=35, scale=scale)
+    out = attend(ptts, b, tree, softcap=cap, out_dtype=out_dtype)
+    b.kv.check()
+    half_out, half_p = b.halves(out_dtype)
+    compare(out, *b.want(softcap=cap, tree=tree, half_out=half_out, half_p=half_p))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_each_refusal_leaves_every_bit(ptts, cuda, dtype):
+    """After every refused call: the caches bit for bit, the lengths of both sides, the output."""
+    import torch
+    b = Batch(ptts, cuda, [5, 9, 0], [2, 1, 1], dtype=dtype, tree=True, seed=20, spare=3)
+    st = [int(s) for s in b.streams]
+    ring, window = sorted(set(range(6)) - set(st))[:2]
+    b.kv.start_ring([ring])
+    b.kv.set_window([window], 4)
+    raw = torch.int16 if dtype == "bf16" else torch.int32
+    bits = lambda: [t.contiguous().view(raw).clone() for t in b.kv.tensors(0)[:2]]  # noqa: E731
+    before, lengths = bits(), b.kv.lengths().copy()
+    out = torch.full((4, 512), 7.0, device=cuda)
+    flat = torch.zeros(4 * 512 + 8, dtype=b.q.dtype, device=cuda)
+    ints = torch.zeros(8, dtype=torch.int32, device=cuda)
+
+    def scored(layer=0, q=b.q, k=b.k, v=b.v, streams=st, rows=(2, 1, 1), **kw):
+        return ptts.attend_scored(b.kv, layer, q, k, v, streams, list(rows), **{"out": out, **kw})
+
+    def tree(parents, streams=st, rows=(2, 1, 1), **kw):
+        return ptts.attend_tree(b.kv, 0, b.q, b.k, b.v, streams, list(rows), parents, out=out, **kw)
+
+    good = b.parents_dev
+    calls = [lambda: scored(layer=1), lambda: scored(layer=-1), lambda: scored(streams=[st[0], st[0], st[1]]),
+             lambda: scored(streams=[st[0], st[1], 6]), lambda: scored(streams=[st[0], st[1], -1]),
+             lambda: scored(rows=(3, 1, 0)), lambda: scored(rows=(5, -1, 0)), lambda: scored(streams=st[:2]),
+             lambda: scored(streams=[st[0], st[1], ring]), lambda: scored(streams=[st[0], st[1], window]),
+             lambda: scored(k=b.k[:, :3].contiguous(), v=b.v[:, :3].contiguous()), lambda: scored(slopes=b.slopes[:4]),
+             lambda: scored(first=ints[:4].long()), lambda: scored(last=ints[::2]), lambda: scored(first=ints[:3]),
+             lambda: scored(out=out[:, ::2]), lambda: scored(out=out.half()), lambda: scored(out=out[:3]),
+             lambda: scored(q=flat[1:1 + 4 * 512].view(4, 8, 64)), lambda: scored(v=flat[1:1 + 4 * 512].view(4, 8, 64)),
+             lambda: scored(out=None, out_dtype="f16"), lambda: scored(slopes=b.slopes.cpu()),
+             lambda: tree(None), lambda: tree(good[:3]), lambda: tree(good.long()), lambda: tree(good.cpu()),
+             lambda: tree(good, streams=[st[0], st[0], st[1]]), lambda: tree(good, streams=[st[0], st[1], ring]),
+             lambda: tree(good, softcap=-2.0), lambda: tree(good, max_period=0.5), lambda: tree(good, first=ints[:3])]
+    calls += [lambda c=c: scored(softcap=c) for c in (-1.0, 1e-38, 1e38, float("nan"), float("inf"))]
+    calls += [lambda p=p: scored(max_period=p) for p in (1.0, -3.0, float("nan"), float("inf"))]
+    calls += [lambda s=s, p=p: b.kv.accept(s, p) for s, p in [
+        ([st[0], st[0]], [[0], [0]]), ([st[0]], [[0], [0]]), ([6], [[0]]), ([-1], [[0]]), ([], []), ([st[1]], [[0, b.capacity - 9]]),
+        ([st[0], ring], [[0], []]), ([window], [[0]]), ([st[0]], [list(range(65))])]]
+    calls += [lambda p=p: b.kv.accept([st[1], st[0]], [[0], p]) for p in ([1, 1], [2, 1], [-1], [0, 64], [0, 1.5])]
+    for i, call in enumerate(calls):
+        with pytest.raises(ptts.PttsError):
+            call()
+        assert all(torch.equal(x, y) for x, y in zip(bits(), before)), i
+        np.testing.assert_array_equal(b.kv.lengths(), lengths)
+        np.testing.assert_array_equal(b.kv.tensors(0)[2].cpu().numpy(), lengths)
+        assert (out == 7.0).all(), i
+    b.kv.check()
+
+
+# ---- f32 caches: scores and weights in f32 --------------------------------------------------------------
+
+def small_windows(q, keys, vals, first, last):
+    """Per row and head over its keys first..last (f64): out, sum_j w_j |v_j - out| (how far a change of the scores
+    moves an element), sum_j w_j |v_j|, and R = sqrt(sum_d (q_d k_d)^2) / 8 of the row's largest (the size of a
+    score's partial sums)."""
+    import torch
+    n, H = q.shape[:2]
+    out, away, size, R = (torch.zeros(n, H, 64, dtype=torch.float64) for _ in range(4))
+    for r in range(n):
+        k, v = keys[first[r]:last[r] + 1].double(), vals[first[r]:last[r] + 1].double()
+        x = q[r].double()[None] * k
+        w = torch.softmax(x.sum(-1) / 8, 0)[..., None]
+        out[r] = (w * v).sum(0)
+        away[r] = (w * (v - out[r]).abs()).sum(0)
+        size[r] = (w * v.abs()).sum(0)
+        R[r] = (x * x).sum(-1).sqrt().amax(0)[:, None] / 8
+    return out, away, size, R
+
+
+def steps_off(got, out, away, size, R):
+    """Root mean square of the errors in units of what f32 gives: a score is a sum of 64 products, each rounded
+    to half a step (2^-24) of partial sums of size R, so 2^-24 sqrt(64) R at most in the mean; a weight's
+    exponential (2 steps of 2^-23), the sums of a few weights and the quotient 2^-22; the output 2^-24."""
+    unit = ((away * R * 2.0 ** -21) ** 2 + (size * 2.0 ** -22) ** 2 + (out * 2.0 ** -24) ** 2).sqrt()
+    return (((got.double() - out) / unit) ** 2).mean().sqrt().item()
+
+
+def pair(x):
+    """x as two bf16 planes."""
+    hi = x.bfloat16().float()
+    return hi + (x - hi).bfloat16().float()
+
+
+@pytest.mark.parametrize("scale,what", [(16.0, "q"), (0.02, "p")])
+def test_the_measure_tells_f32_from_bf16_pairs(scale, what):
+    """f32 arithmetic stays under 1 in the mean, a bf16 pair in place of q (large scores) or of the weights
+    (scores near 0) does not: 2^-18 of a value against 2^-21 and 2^-22."""
+    import torch
+    g = torch.Generator().manual_seed(1)
+    n = 200
+    q, keys, vals = torch.randn(n, 8, 64, generator=g) * scale, *(torch.randn(n + 3, 8, 64, generator=g) for _ in range(2))
+    first, last = np.arange(n), np.arange(n) + 3
+    want = small_windows(q, keys, vals, first, last)
+
+    def f32(q, p_of):
+        out = torch.zeros(n, 8, 64)
+        for r in range(n):
+            s = torch.einsum("hd,thd->th", q[r], keys[r:r + 4]) / 8
+            e = torch.exp(s - s.amax(0))
+            out[r] = torch.einsum("th,thd->hd", p_of(e), vals[r:r + 4]) / e.sum(0)[:, None]
+        return steps_off(out, *want)
+
+    assert f32(q, lambda p: p) < 0.7
+    assert f32(pair(q) if what == "q" else q, pair if what == "p" else (lambda p: p)) > 1.4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [16.0, 0.02])
+@pytest.mark.parametrize("kind", ["tokens", "prompts", "trees"])
+def test_f32_caches_hold_scores_and_weights_in_f32(ptts, cuda, kind, scale):
+    """Windows of 4 keys, so that long sums do not hide what a pair of bf16s would lose; a tree of one chain is a
+    prompt. Under 1 in the units of steps_off."""
+    rows = {"tokens": [1] * 150, "prompts": [70, 33], "trees": [64, 40]}[kind]
+    cached = [3 + 7 * i % 90 for i in range(len(rows))]
+    b = Batch(ptts, cuda, cached, rows, dtype="f32", tree=kind == "trees", seed=36, scale=scale,
+              parents=[list(range(-1, n - 1)) for n in rows])
+    pos = np.concatenate(b.positions())
+    out = attend(ptts, b, kind == "trees", first=b.dev((pos - 3).astype(np.int32)), max_period=0.0)
+    b.kv.check()
+    off, at = [], 0
+    kt, vt, _ = b.kv.tensors(0)
+    for st, L, n in zip(b.streams, b.cached, b.rows):
+        p = np.arange(L, L + n)
+        want = small_windows(b.q[at:at + n].cpu(), kt[int(st)].cpu(), vt[int(st)].cpu(), p - 3, p)
+        off.append(steps_off(out[at:at + n].cpu().reshape(n, 8, 64), *want) ** 2 * n)
+        at += n
+    assert (sum(off) / at) ** 0.5 < 1.0
