@@ -549,3 +549,45 @@ def test_f32_caches_hold_scores_and_weights_in_f32(ptts, cuda, kind, scale):
         off.append(steps_off(out[at:at + n].cpu().reshape(n, 8, 64), *want) ** 2 * n)
         at += n
     assert (sum(off) / at) ** 0.5 < 1.0
+
+
+# ---- keys that a row does not see ---------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", [30.0, -1e3, float("inf"), float("nan")])
+@pytest.mark.parametrize("rule", [{}, {"softcap": 30.0}, {"softcap": 50.0}, {"softcap": 50.0, "slopes": True}, {"softcap": 200.0},
+                                  {"softcap": 0.5}], ids=str)
+@pytest.mark.parametrize("dtype,out_dtype", [("bf16", "bf16"), ("bf16", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("kind", ["prompts", "rows", "tokens", "trees"])
+def test_keys_that_a_row_does_not_see_change_no_bit_of_it(ptts, cuda, kind, dtype, out_dtype, rule, what):
+    """Two documents in a stream (a tree: a node beside the others): the first one's keys and values, the call's
+    own among them, and the slots behind the call's rows are replaced; the second one's rows keep their bits."""
+    import torch
+    cached, rows, tree = {"prompts": (200, 150, False), "rows": (3000, 40, False), "tokens": (900, 1, False),
+                          "trees": (700, 30, True)}[kind]
+    cut = {"prompts": 237, "rows": 3011, "tokens": 333, "trees": 411}[kind]  # where the second document begins
+    parents = [[-1] + [0 if i < 8 else i - 7 for i in range(1, rows)]]  # node 5: its line is 5, 12, 19, 26
+    outs = []
+    for changed in (False, True):
+        b = Batch(ptts, cuda, [cached], [rows], dtype=dtype, tree=tree, parents=parents, seed=51)
+        line = {i for i, l in enumerate(lineages(parents[0])[1]) if 5 in l} if tree else set()
+        pos = cached + (np.array(lineages(parents[0])[0]) if tree else np.arange(rows))
+        if tree:
+            keep, first = [i for i in range(rows) if i not in line], np.full(rows, cut)
+        else:
+            keep, first = [i for i in range(rows) if pos[i] >= cut], np.where(pos >= cut, cut, 0)
+        kt, vt, _ = b.kv.tensors(0)
+        st = int(b.streams[0])
+        kt[st, cached:], vt[st, cached:] = 0.0, 0.0
+        if changed:
+            for t in (kt, vt):
+                t[st, :min(cut, cached)] *= what
+                t[st, cached + rows:] = what
+            away = [5] if tree else [i for i in range(rows) if pos[i] < cut]
+            for t in (b.k, b.v):
+                t[away] *= what
+        slopes = b.slopes if rule.get("slopes") else None
+        args = dict(softcap=rule.get("softcap", 0.0), slopes=slopes, first=b.dev(first.astype(np.int32)), out_dtype=out_dtype)
+        outs.append(attend(ptts, b, tree, **args)[keep].clone())
+        b.kv.check()
+    assert torch.isfinite(outs[0]).all() and torch.equal(outs[0], outs[1])

@@ -14,19 +14,20 @@ __device__ __forceinline__ float score_exp2(float x) {
     return y;
 }
 
-// tanh in f32 for the lanes of a warp, all of them here: y p(y^2), the best fit of degree 5 on
-// |y| <= 1/2 (largest error 7.4e-11, below f32's own rounding), where no lane is past it, else tanhf.
-__device__ __forceinline__ float warp_tanh(float y) {
-    if (__any_sync(0xffffffffu, fabsf(y) > 0.5f)) return tanhf(y);
+// tanh in f32: y p(y^2), the best fit of degree 5, on |y| <= 1/2 (largest error 2.1e-9 with its constants
+// in f32, a seventh of f32's half step there), else tanhf. Each lane by its own y: a vote of the warp
+// would let a key that a row does not see choose the form, and with it the last bits, of one that it sees.
+__device__ __forceinline__ float f32_tanh(float y) {
+    if (fabsf(y) > 0.5f) return tanhf(y);
     const float z = y * y;
     return y * fmaf(fmaf(fmaf(fmaf(fmaf(-0.00646002789f, z, 0.0211690968f), z, -0.0538669695f), z, 0.133326121f), z,
                          -0.333333112f), z, 0.999999998f);
 }
 
-// u * log2(e) of a score s = q . k / 8 at a distance (either sign), in f32 (whole warps): small scores
-// under a large cap keep their digits. `inv_cap` = 1 / cap.
+// u * log2(e) of a score s = q . k / 8 at a distance (either sign), in f32: small scores under a large cap
+// keep their digits. `inv_cap` = 1 / cap.
 __device__ __forceinline__ float score_exact(float s, float cap, float inv_cap, float slope, int distance) {
-    if (cap > 0.f) s = cap * warp_tanh(s * inv_cap);
+    if (cap > 0.f) s = cap * f32_tanh(s * inv_cap);
     return (s - slope * (float)abs(distance)) * kScoreLog2e;
 }
 
@@ -37,13 +38,16 @@ __device__ __forceinline__ float cap_exact(float x, float cap) {
 }
 // Fast: y = s / cap, for N scores of a thread. tanh(y) = y p(y^2) with the polynomial of degree 3
 // that fits it best (least largest error, 3.6e-6) on |y| <= 3/4, fitted to numpy's tanh by reweighted
-// least squares; where some score of the warp is past that, tanh(y) = 1 - 2 / (1 + e^2y) by one exp2
+// least squares; where some score is past that, tanh(y) = 1 - 2 / (1 + e^2y) by one exp2
 // and one reciprocal, whose difference cancels near 0 (an absolute error near 2^-20). Either moves a
 // weight by less than 2^-10 for cap <= kScoreFastCap, a quarter of bf16's own half step of 2^-8.
 // On the packed FMAs the polynomial costs 5 pipe cycles a score, the other form 2 of the 3 operations
 // at exp2's rate (8 cycles each) that would then bound a capped softmax.
-template <int N>
-__device__ __forceinline__ void cap_fast(float* y, float cap) {
+// No row's bits depend on a key that it does not see. Either each thread chooses its form, whose scores are
+// one key's, or one row's with those that it does not see set to 0 by the caller; or (VOTE) the warp does,
+// the polynomial only where all its rows see all its keys (`all_seen`).
+template <int N, bool VOTE>
+__device__ __forceinline__ void cap_fast(float* y, float cap, bool all_seen = true) {
     const float c = cap * kScoreLog2e;
     float most = 0.f;
 #pragma unroll
@@ -51,7 +55,9 @@ __device__ __forceinline__ void cap_fast(float* y, float cap) {
         const float2 v = make_float2(y[i], y[i + 1]), z = __fmul2_rn(v, v);
         asm("max.f32 %0, %0, %1, %2;" : "+f"(most) : "f"(z.x), "f"(z.y));
     }
-    if (__all_sync(0xffffffffu, most <= 0.5625f)) {  // a NaN score passes, and stays NaN
+    bool small = most <= 0.5625f;  // a NaN score passes, and stays NaN
+    if (VOTE) small = all_seen && __all_sync(0xffffffffu, small);
+    if (small) {
         const float2 k0 = make_float2(0.999955601f * c, 0.999955601f * c), k1 = make_float2(-0.332227634f * c, -0.332227634f * c),
                      k2 = make_float2(0.125770911f * c, 0.125770911f * c), k3 = make_float2(-0.0337782684f * c, -0.0337782684f * c);
 #pragma unroll
