@@ -591,3 +591,25 @@ def test_keys_that_a_row_does_not_see_change_no_bit_of_it(ptts, cuda, kind, dtyp
         outs.append(attend(ptts, b, tree, **args)[keep].clone())
         b.kv.check()
     assert torch.isfinite(outs[0]).all() and torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [2.0 ** -35, 2.0 ** 70, 2.0 ** 100])
+@pytest.mark.parametrize("cap,to", [(20.0, 1), (20.0, -1), (32.0, 1), (32.0, -1), (40.0, 1), (40.0, -1), (50.0, 1), (0.0, 1)])
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("kind", ["rows", "prompts", "trees", "tokens"])
+def test_values_of_any_size(ptts, cuda, kind, slopes, cap, to, size):
+    """Values far from 1 beside scores at the cap (to: at its upper or lower end): finite, and in bounds relative to
+    the values (test_scores.py's; its weights are relative too)."""
+    import torch
+    cached, rows, tree = CALLS[kind]
+    b = Batch(ptts, cuda, cached, rows, tree=tree, seed=52)
+    kt, vt, _ = b.kv.tensors(0)
+    common = torch.randn(8, 64, device=cuda)  # in every q and key: scores of about `to` x 100
+    b.q.copy_(b.q * 0.2 + common * 10), b.k.copy_(b.k * 0.2 + common * to)
+    kt.copy_(kt * 0.2 + common * to), vt.mul_(size), b.v.mul_(size)
+    rules = dict(softcap=cap, slopes=b.slopes if slopes else None, max_period=0.0)
+    out = attend(ptts, b, tree, out_dtype="bf16", **rules)
+    b.kv.check()
+    want, bound = b.want(tree=tree, half_out=2.0 ** -8, half_p=2.0 ** -8, **rules)
+    compare(out / size, want / size, bound / size)

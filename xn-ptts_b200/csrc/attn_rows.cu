@@ -234,7 +234,8 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
                 R->hi[key] = hi;
                 R->pos[key] = (float)(pos - origin);
                 R->lineage[key] = there && a.rows.lineage ? a.rows.lineage[row] : 0;
-                // BOUNDED: exp2 against the row's greatest bias (a node sees positions lo .. its own). Else the
+                // BOUNDED: exp2 against the row's greatest bias (a node sees positions lo .. its own), and
+                // three quarters of the cap, which cap_fast takes off. Else the
                 // row's first scores set m.
                 R->m[key] = BOUNDED && biased ? most_bias(slope, pos, lo, a.rows.lineage ? min(hi, pos) : hi) : 0.f;
                 R->has[key] = lo > hi;
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
                     for (int g = 0; g < 4; ++g) {
                         if (g >= groups) continue;
                         float* x = s + 16 * g;
-                        if (CAP == kCapFast) cap_fast<16, false>(x, a.rule.cap);  // (a vote of the warp: tree_batch 113 us, 107 so)
+                        if (CAP == kCapFast) cap_fast<16, false, BOUNDED>(x, a.rule.cap);  // (a vote of the warp: tree_batch 113 us, 107 so)
                         if (CAP == kCapExact) {
 #pragma unroll
                             for (int j = 0; j < 16; ++j) x[j] = cap_exact(x[j], a.rule.cap);
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(kThreadsR, 1) score_rows_kernel(ScoreRowsArgs 
 #pragma unroll
                             for (int j = 0; j < 16; ++j) x[j] = bits >> j & 1 ? x[j] : -INFINITY;
                         }
-                        // From here on the scores are past their rows' maxima (or BOUNDED's references, 0 without a bias).
+                        // From here on the scores are past their rows' maxima (or BOUNDED's references, m = 0 without a bias).
                         if (!BOUNDED || biased) {
 #pragma unroll
                             for (int j = 0; j < 16; j += 4) {

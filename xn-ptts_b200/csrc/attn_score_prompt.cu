@@ -18,8 +18,8 @@
 // sharing K and V: 167 and 373.
 // Two threads a row and two CTAs an SM make four softmax warps a scheduler, which fill each other's
 // waits (with a thread a row, half as many, the issue slots were 35 to 46 % used). Where a cap up to
-// kScoreBoundedCap bounds the scores there is no maximum: exp2 runs against the row's greatest
-// bias, which a score passes by at most cap x log2(e) < 58 either way. Items run from the last keys to
+// kScoreBoundedCap bounds the scores there is no maximum: exp2 runs against the row's greatest bias and
+// three quarters of the cap, which a score is from 81 below to 12 above. Items run from the last keys to
 // the first: a causal row's nearest keys, whose bias is the least, set the maximum at once.
 //
 // f32 outputs hold P as a bf16 hi/lo pair over the columns of S (its next item waits for P V);
@@ -109,9 +109,9 @@ __device__ __forceinline__ void rules(float* s, float cap, float slope, int ahea
 #pragma unroll
             for (int j = 0; j < 32; ++j) s[j] = seen >> j & 1 ? s[j] : 0.f;
         }
-        cap_fast<32, false>(s, cap);
+        cap_fast<32, false, true>(s, cap);
     }
-    if (CAP == kCapFast && !BOUNDED) cap_fast<32, true>(s, cap, !some);
+    if (CAP == kCapFast && !BOUNDED) cap_fast<32, true, false>(s, cap, !some);
     if (CAP == kCapExact) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) s[j] = cap_exact(s[j], cap);

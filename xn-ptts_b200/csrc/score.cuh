@@ -46,7 +46,10 @@ __device__ __forceinline__ float cap_exact(float x, float cap) {
 // No row's bits depend on a key that it does not see. Either each thread chooses its form, whose scores are
 // one key's, or one row's with those that it does not see set to 0 by the caller; or (VOTE) the warp does,
 // the polynomial only where all its rows see all its keys (`all_seen`).
-template <int N, bool VOTE>
+// LESS: less three quarters of the cap, for weights without a maximum. They then lie within 2^-81 and 2^12
+// (kScoreBoundedCap), so that values up to 2^94 of a million keys, and down to 2^-45, stay among f32's normal
+// numbers beside scores at either end of the cap.
+template <int N, bool VOTE, bool LESS>
 __device__ __forceinline__ void cap_fast(float* y, float cap, bool all_seen = true) {
     const float c = cap * kScoreLog2e;
     float most = 0.f;
@@ -59,11 +62,13 @@ __device__ __forceinline__ void cap_fast(float* y, float cap, bool all_seen = tr
     if (VOTE) small = all_seen && __all_sync(0xffffffffu, small);
     if (small) {
         const float2 k0 = make_float2(0.999955601f * c, 0.999955601f * c), k1 = make_float2(-0.332227634f * c, -0.332227634f * c),
-                     k2 = make_float2(0.125770911f * c, 0.125770911f * c), k3 = make_float2(-0.0337782684f * c, -0.0337782684f * c);
+                     k2 = make_float2(0.125770911f * c, 0.125770911f * c), k3 = make_float2(-0.0337782684f * c, -0.0337782684f * c),
+                     less = make_float2(-0.75f * c, -0.75f * c);
 #pragma unroll
         for (int i = 0; i < N; i += 2) {
             const float2 v = make_float2(y[i], y[i + 1]), z = __fmul2_rn(v, v);
-            const float2 t = __fmul2_rn(v, __ffma2_rn(__ffma2_rn(__ffma2_rn(k3, z, k2), z, k1), z, k0));
+            const float2 p = __ffma2_rn(__ffma2_rn(__ffma2_rn(k3, z, k2), z, k1), z, k0);
+            const float2 t = LESS ? __ffma2_rn(v, p, less) : __fmul2_rn(v, p);
             y[i] = t.x;
             y[i + 1] = t.y;
         }
@@ -72,7 +77,7 @@ __device__ __forceinline__ void cap_fast(float* y, float cap, bool all_seen = tr
         for (int i = 0; i < N; ++i) {
             float r;
             asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + score_exp2(2.f * kScoreLog2e * y[i])));
-            y[i] = fmaf(-2.f * c, r, c);
+            y[i] = fmaf(-2.f * c, r, LESS ? 0.25f * c : c);
         }
     }
 }

@@ -113,8 +113,9 @@ void launch_score_f32(const ScoreF32Args& a, cudaStream_t s);
 // without a cap).
 enum { kCapNone = 0, kCapFast = 1, kCapExact = 2 };
 constexpr float kScoreFastCap = 128.f;
-// Caps this small bound the scores: 40 log2(e) < 58, and weights and sums of 2^58 stay far inside f32 and bf16.
-constexpr float kScoreBoundedCap = 40.f;
+// Caps this small bound the scores well inside f32's and bf16's exponents (32 log2(e) < 47): no maximum is
+// kept (see cap_fast).
+constexpr float kScoreBoundedCap = 32.f;
 inline int score_cap_mode(float cap, bool out_f32) {
     return cap == 0.f ? kCapNone : (!out_f32 && cap >= 1e-3f && cap <= kScoreFastCap ? kCapFast : kCapExact);
 }
