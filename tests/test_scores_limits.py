@@ -613,3 +613,47 @@ def test_values_of_any_size(ptts, cuda, kind, slopes, cap, to, size):
     b.kv.check()
     want, bound = b.want(tree=tree, half_out=2.0 ** -8, half_p=2.0 ** -8, **rules)
     compare(out / size, want / size, bound / size)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out_dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,tree", [(1, False), (1, True), (2, False), (2, True), (64, True), (130, False)])
+def test_a_cache_of_one_stream_filled_by_one_call(ptts, cuda, rows, tree, dtype, out_dtype):
+    """No slot beside the call's own rows; one-key rows give the key's value."""
+    import torch
+    kv = ptts.KvState(1, 1, rows, dtype=dtype)
+    t = torch.bfloat16 if dtype == "bf16" else torch.float32
+    q, k, v = (torch.randn(rows, 8, 64, device=cuda).to(t) for _ in range(3))
+    args = (kv, 0, q, k, v, [0], [rows])
+    rules = dict(softcap=30.0, slopes=torch.full((8,), 0.5, device=cuda), out_dtype=out_dtype)
+    if tree:  # roots: each sees itself
+        out = ptts.attend_tree(*args, torch.full((rows,), -1, dtype=torch.int32, device=cuda), **rules)
+        assert torch.equal(out.view(rows, 8, 64), v.to(out.dtype))
+    else:
+        out = ptts.attend_scored(*args, **rules)
+        # bf16 outputs of prompts: a weight rounded to bf16 (2^-8) over its sum in f32, then the output's rounding
+        # (2^-8, of what that left). Else the weight is 1, exactly.
+        slack = (1 + 2.0 ** -8) ** 2 - 1 if rows > 1 and dtype == out_dtype == "bf16" else 0.0
+        want = v[0].to(out.dtype).double()
+        assert ((out[0].view(8, 64).double() - want).abs() <= slack * want.abs()).all()
+        assert torch.isfinite(out).all()
+    kv.check()
+    with pytest.raises(ptts.PttsError):
+        kv.advance([0], [rows + 1])
+    kv.accept([0], [list(range(min(rows, 64)))])
+    kv.check()
+    assert kv.lengths()[0] == min(rows, 64) and torch.equal(kv.tensors(0)[1][0].to(t), v)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,out_dtype", [("bf16", "bf16"), ("bf16", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("kind", list(CALLS))
+def test_the_same_call_gives_the_same_bits(ptts, cuda, kind, dtype, out_dtype):
+    import torch
+    cached, rows, tree = CALLS[kind]
+    b = Batch(ptts, cuda, [c + 2000 for c in cached], rows, dtype=dtype, tree=tree, seed=53)
+    for rules in ({}, {"softcap": 30.0}, {"softcap": 50.0, "slopes": b.slopes}):
+        outs = [attend(ptts, b, tree, out_dtype=out_dtype, **rules).clone() for _ in range(5)]
+        assert all(torch.equal(o, outs[0]) for o in outs)
+    b.kv.check()
