@@ -224,7 +224,12 @@ int ptts_b200_attend(ptts_b200_kv* kv, int layer, const void* q, const void* k, 
  *   t_j = softcap * tanh(s_j / softcap)    (s_j where softcap is 0)
  *   u_j = t_j - slopes[head] * |p - j|     (t_j where slopes is NULL)
  *   out = sum_j exp(u_j) v_j / sum_j exp(u_j), and zeros for a row that sees nothing.
- * Keys that a row does not see never reach its output, whatever they hold (NaN included).
+ * Keys that a row does not see never reach its output, not a bit of it, whatever they hold (NaN included).
+ * Scores, biases and sums are f32: where slope x distance is large the bias has f32's step (2^-24 of it),
+ * so rows that see far keys alone lose digits of their weights. Prompts and trees on bf16 caches hold q in a
+ * pair of bf16s (2^-17) and the weights exp(u), for their product with v, in a pair for f32 outputs and in
+ * one bf16 for bf16 outputs (2^-8 of each weight, beside the output's own rounding). Single tokens and f32
+ * caches hold both in f32.
  * ------------------------------------------------------------------------------------- */
 typedef struct {
     float softcap;         /* within 1e-30 .. 1e30, or 0 for none */
@@ -240,7 +245,8 @@ typedef struct {
  * max_period 0 leaves q and k unrotated (for a distance bias in place of RoPE).
  * q, k, v and out are aligned to 16 bytes. Streams are appended streams (rings and windowed
  * streams are refused with PTTS_B200_ERR_UNSUPPORTED), and the call cannot be captured in a CUDA
- * graph (PTTS_B200_ERR_STATE): it plans from the host's lengths. Lengths are not advanced.
+ * graph (PTTS_B200_ERR_STATE): it plans from the host's lengths, and its scratch is allocated when a call
+ * needs more. Lengths are not advanced.
  * Rows are placed by the device's lengths. Where those are not the host's any more (a caller's graph
  * that advances, a caller that writes them) a sequence that does not fit its stream there is refused on
  * the device (PTTS_B200_DEVERR_CAPACITY in ptts_b200_kv_check): nothing is written to its slots and its

@@ -518,6 +518,8 @@ def attend_scored(kv: KvState, layer: int, q, k, v, streams: Sequence[int], rows
     softcap), biased by -slopes[head] * |position - key position| (slopes f32 [H]), each row seeing
     the positions first..last (int32 [n_rows]; None: 0 and its own position). All on the cache's
     device. max_period 0: no rotation. A row that sees nothing is zeros.
+    out_dtype "bf16" rounds more than the output on bf16 caches: prompts' softmax weights are then held in
+    one bf16 for the product with v (2^-8 of each); with "f32", the default and the slower, in two.
 
     Masks as spans, for a row at position p: documents packed in one stream, first = the start of
     p's document; a prefix that sees itself whole, last = max(p, prefix - 1); a window of w,
@@ -532,7 +534,8 @@ def attend_tree(kv: KvState, layer: int, q, k, v, streams: Sequence[int], rows: 
     """Attention of drafted trees over the cache (see ptts_b200_attend_tree): rows[i] nodes (at most
     64) on stream streams[i]; parents int32 [n_rows], a node's parent within its sequence (below its
     own index) or -1. A node sees the cached rows, its ancestors and itself, at position length +
-    depth; its k and v go to slot length + index. KvState.accept keeps a path."""
+    depth; its k and v go to slot length + index. KvState.accept keeps a path. out_dtype as in
+    attend_scored."""
     return _attend_rules(kv, layer, q, k, v, streams, rows, parents, True, softcap, slopes, first, None, max_period,
                          out_dtype, out, stream)
 

@@ -5,7 +5,7 @@
 // once). A thread owns one 16-byte column of a (stream, block, K or V) and takes the path's rows in
 // order, kBatch loads ahead of their stores: nodes rise, so node[j] >= j and no store comes before
 // a load that needs its slot, and columns share no byte, so no thread waits for another. Measured (one
-// B200): 512 paths in 9 layers, 12.5 us on the GPU.
+// B200): 512 paths in 9 layers, 14 us on the GPU, 1 to 2 of them a stream's CTAs counting one another.
 #include "common.cuh"
 #include "score.h"
 

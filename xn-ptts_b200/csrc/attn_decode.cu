@@ -32,7 +32,7 @@
 // With score rules (SCORED): the same split and ring over each row's visible span, its scores capped
 // and biased in f32 between the dot product and the running maximum (see score.h). One lane computes a
 // row's rules and exponential, so capped scores keep the copies as the bound: 256 ragged streams of 64-2048
-// keys, one token each, 6.06 TB/s for a whole call (with every lane computing them, 5.1).
+// keys, one token each, 6.0 TB/s for a whole call (with every lane computing them, 5.1).
 #include "common.cuh"
 #include "kernels.h"
 #include "score.cuh"

@@ -24,8 +24,8 @@
 //                   are in registers.
 //   warp 10         one lane copies the heads' Q tiles and K and V items by TMA, two slots each.
 // Measured (one B200, 8 heads, bf16): 128 streams of 64-2048 cached rows with trees of 8-64 nodes, cap 30,
-// 108 us a call, about 85 of them this kernel (an item 1.2 us at 16 rows, 2.1 at 64, 1.46 at HBM's rate; a
-// block's start and end 4-6 that nothing overlaps); 4 full trees over 20000-33000 rows, 78 us a call. Rows
+// 107 us a call, about 85 of them this kernel (an item 1.2 us at 16 rows, 2.1 at 64, 1.46 at HBM's rate; a
+// block's start and end 4-6 that nothing overlaps); 4 full trees over 20000-33000 rows, 77 us a call. Rows
 // as M on mma.sync took 213 and 125 where this form then took 129 and 87.
 // A block inside one CTA's range is written at once; the pieces of a cut block leave (max, sum, acc)
 // records that a second kernel joins, one warp per row and head: 64 rows x 8 heads are too many for

@@ -12,8 +12,8 @@
 //              item's S starts as soon as the softmax holds this one's in registers.
 //   warp 9     one lane copies each head's Q tile and each item's K and V (128 keys) by TMA, K and V
 //              in two-slot rings, so the next head's data come during this head's last item.
-// Measured (one B200, bf16): 96 streams of 200-900 rows in documents, cap 30, 8 heads, 145 us (issue 37 %,
-// tensor 19 %); 4 streams of 3900-4096 rows, 16 heads, a distance bias, 300 us (exp2 43 %, issue 48 %,
+// Measured (one B200, bf16): 96 streams of 200-900 rows in documents, cap 30, 8 heads, 140 us (issue 39 %,
+// tensor 20 %); 4 streams of 3900-4096 rows, 16 heads, a distance bias, 300 us (exp2 43 %, issue 48 %,
 // tensor 35 %: 430 TFLOP/s of the products that count). A thread a row: 172 and 318; two tiles a CTA
 // sharing K and V: 167 and 373.
 // Two threads a row and two CTAs an SM make four softmax warps a scheduler, which fill each other's
