@@ -178,9 +178,10 @@ __device__ __forceinline__ void plan(const ScorePlanArgs& a, const int32_t* list
     const int sq = seq_of_warp(a, offsets, r, lane), row0 = offsets[sq];
     const int rows = offsets[sq + 1] - row0, sid = list[sq];
     const bool known = sid >= 0 && sid < a.num_streams;
-    const int base = known ? a.lengths[sid] : 0;
+    const int length = known ? a.lengths[sid] : 0;
+    bool good = known && fits(a, length, rows);  // the whole sequence: its rows see each other's slots
+    const int base = good ? length : 0;          // a refused row's numbers mean nothing, and stay small
     const int node = r - row0, slot = base + node;
-    bool good = known && fits(a, base, rows);  // the whole sequence: its rows see each other's slots
     if (!good && lane == 0) set_error(a.err, known ? DEV_ERR_CAPACITY : DEV_ERR_BOUNDS);
     int pos = slot, lo = 0, hi = -1;
     if (good) row_span(a, r, base, row0, rows, lo, hi);
