@@ -172,8 +172,9 @@ bool launch_score_prompt(const ScorePromptArgs& a, cudaStream_t s);
 
 // Acceptance: per stream the accepted nodes' rows move from slot len + node[j] to len + j, in
 // every layer and head group, and the length becomes len + their number. A stream whose length on the
-// device is not `len` is refused there (DEV_ERR_BOUNDS) and stays as it is. Nodes rise, so node[j] >= j. The lists are one array of int32 (host or device): streams [n], lengths before
-// [n], offsets into the nodes [n + 1], nodes.
+// device is not `len` is refused there (DEV_ERR_BOUNDS) and stays as it is. Nodes rise, so node[j] >= j.
+// The lists are one array of int32 (host or device): streams [n], lengths before [n], offsets into the
+// nodes [n + 1], nodes.
 constexpr int kAcceptInline = 512;
 struct AcceptInline {  // a short list rides in the launch's parameters
     int32_t list[kAcceptInline];
