@@ -657,3 +657,24 @@ def test_the_same_call_gives_the_same_bits(ptts, cuda, kind, dtype, out_dtype):
         outs = [attend(ptts, b, tree, out_dtype=out_dtype, **rules).clone() for _ in range(5)]
         assert all(torch.equal(o, outs[0]) for o in outs)
     b.kv.check()
+
+
+@pytest.mark.gpu
+def test_caches_on_streams_of_their_own_at_once(ptts, cuda):
+    """Four caches, each with another kernel's call on its own stream, several times over without a wait: the bits
+    of the same calls one after another."""
+    import torch
+    jobs = [(Batch(ptts, cuda, *CALLS[k][:2], dtype=dtype, tree=CALLS[k][2], seed=54 + i), CALLS[k][2])
+            for i, (k, dtype) in enumerate([("prompts", "bf16"), ("trees", "bf16"), ("tokens", "bf16"), ("prompts", "f32")])]
+    rules = dict(softcap=30.0, out_dtype="bf16")
+    alone = [attend(ptts, b, tree, **rules) for b, tree in jobs]
+    outs = [[torch.empty_like(a) for _ in range(20)] for a in alone]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for (b, tree), s, o in zip(jobs, streams, outs):
+            attend(ptts, b, tree, **{**rules, "out": o[i], "stream": s})
+    torch.cuda.synchronize()
+    for (b, _), a, o in zip(jobs, alone, outs):
+        b.kv.check()
+        assert all(torch.equal(x, a) for x in o)
